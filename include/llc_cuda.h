@@ -158,6 +158,93 @@ typedef struct LlcEmbedNormParams {
 } LlcEmbedNormParams;
 int llc_cuda_embed_norm(const LlcEmbedNormParams* p, void* stream);
 
+/* Rotary positions: out[t,h,:] is x[t,h,:] with `pairs` pairs of its elements turned, pair i by the angle
+ * a = positions[axis(i)][t] * inv_freq[i]:  (x, y) -> (x cos a - y sin a, x sin a + y cos a).  Pair i is elements
+ * (i, i + pairs), or (2 i, 2 i + 1) when interleaved; elements from 2 * pairs on are copied.  The pairs are dealt out to the
+ * axes in order, sections[0] to axis 0 and so on (time, height and width of a video, say); the sections add up to pairs.
+ * Angles are computed in 64 bits, the turn in 32, one rounding at the store.  x and out have unit stride along d; out may
+ * be x itself (same address, same strides), any other overlap is the caller's error.  No counterpart in the reference. */
+#define LLC_ROTARY_MAX_AXES 4
+typedef struct LlcRotaryParams {
+  const void* x; void* out;
+  const void* positions;       /* [axes, tokens], unit stride along tokens */
+  const double* inv_freq;      /* [pairs] */
+  int32_t dtype;               /* LLC_FLOAT32, LLC_BFLOAT16 or LLC_FLOAT16 */
+  int32_t pos_dtype;           /* LLC_INT32 or LLC_INT64 */
+  int64_t tokens, heads, d, pairs;
+  int64_t x_st, x_sh, o_st, o_sh;   /* strides of a token and of a head */
+  int64_t pos_sa;                   /* stride of an axis of positions */
+  int32_t axes;                     /* 1 to LLC_ROTARY_MAX_AXES */
+  int32_t interleaved;
+  int32_t sections[LLC_ROTARY_MAX_AXES];
+} LlcRotaryParams;
+int llc_cuda_rotary(const LlcRotaryParams* p, void* stream);
+
+/* ---- Paged key / value cache ----------------------------------------------------------------------------------------
+ * A cache is a pool of pages of page_size token slots, k_cache and v_cache of logical shape
+ * [num_pages, page_size, kv_heads, d] with any strides along the first three dims.  A batch of sequences is described by
+ * three int32 arrays on the device, so that a captured graph can be replayed with other lengths:
+ *   page_table [batch, table_width]  slot j of sequence b is slot j % page_size of page page_table[b][j / page_size]
+ *   q_start    [batch + 1]           rows q_start[b] .. q_start[b+1]-1 of q, k and v are sequence b's new tokens
+ *   kv_len     [batch]               tokens of sequence b in the cache, its new ones included: the i-th of n new tokens
+ *                                    has place kv_len[b] - n + i
+ * Rows from q_start[batch] on belong to nobody and are left as they were.  A length beyond the table's reach counts as the
+ * reach, a negative one as 0.  Page numbers outside [0, num_pages) are never followed.
+ *
+ * llc_cuda_kv_append writes the new tokens' keys and values into their slots, the keys turned by their rotary angles when
+ * inv_freq is not NULL, and writes the queries, turned the same way, to q_out when q is not NULL.  positions NULL: every
+ * axis is the token's place.  A token whose page number is outside [0, num_pages) or whose place is outside the table
+ * (or negative) is not stored and is counted in *bad_pages when that is not NULL (a device int32); its query is turned
+ * all the same.  Two tokens of a call must not have the same slot.  No counterpart in the reference. */
+typedef struct LlcKvAppendParams {
+  const void* k; const void* v; void* k_cache; void* v_cache;
+  const void* q; void* q_out;          /* optional */
+  const int32_t* page_table; const int32_t* q_start; const int32_t* kv_len;
+  const void* positions;               /* optional: [axes, tokens], unit stride along tokens */
+  const double* inv_freq;              /* optional: [pairs] */
+  int32_t* bad_pages;                  /* optional */
+  int32_t dtype;                       /* all tensors: LLC_FLOAT32, LLC_BFLOAT16 or LLC_FLOAT16 */
+  int32_t pos_dtype;                   /* LLC_INT32 or LLC_INT64 */
+  int64_t tokens, batch, heads, kv_heads, d, pairs;
+  int64_t num_pages, page_size, table_width, table_s0;
+  int64_t q_st, q_sh, qo_st, qo_sh, k_st, k_sh, v_st, v_sh;
+  int64_t kc_sp, kc_sn, kc_sh, vc_sp, vc_sn, vc_sh;   /* strides of a page, a slot and a head */
+  int64_t pos_sa;
+  int32_t axes, interleaved;
+  int32_t sections[LLC_ROTARY_MAX_AXES];
+} LlcKvAppendParams;
+int llc_cuda_kv_append(const LlcKvAppendParams* p, void* stream);
+
+/* out[t,h,:] = sum_j w_j v_j, w = softmax over the visible j of scale * q[t,h,:] . k_j, for the new tokens t of a ragged
+ * batch over a paged cache that holds their keys and values already (llc_cuda_kv_append); query head h reads key head
+ * h / (heads / kv_heads).  A token at place p sees the keys j <= p; with window > 0 only those with p - j < window, and the
+ * first `sinks` keys of the sequence besides.  A token that sees nothing (kv_len smaller than its place asks for) gets zeros.
+ * A slot whose page number is outside [0, num_pages) reads as zeros (key and value) and each such page that a query sees is
+ * counted in *bad_pages (at least once, or more often) when that is not NULL.  Nothing else of the cache is read into the
+ * result: slots past kv_len, pages before the window and unused pages may hold anything.
+ * max_q: at least the largest number of new tokens of a sequence; a sequence that has more is left out.
+ * f32, bf16 and f16, all tensors alike, unit stride along d, d <= 256.  bf16 and f16 with d 64 or 128, page_size a power of
+ * two >= 16, strides of 16 bytes' multiples and 16-byte aligned pointers run on the tensor cores, everything else
+ * (f32, other head sizes, pages and strides) on a kernel of plain multiply-adds.
+ * workspace: scratch for joining sums over parts of the keys, llc_cuda_paged_attention_workspace bytes, 16-byte aligned,
+ * contents arbitrary; NULL (or too small) disables the split.  Launches that share one must not overlap on the GPU. */
+typedef struct LlcPagedAttentionParams {
+  const void* q; const void* k_cache; const void* v_cache; void* out;
+  const int32_t* page_table; const int32_t* q_start; const int32_t* kv_len;
+  int32_t* bad_pages;                  /* optional */
+  int32_t dtype;
+  float scale;
+  int64_t tokens, batch, heads, kv_heads, d, max_q;
+  int64_t num_pages, page_size, table_width, table_s0;
+  int64_t q_st, q_sh, o_st, o_sh;
+  int64_t kc_sp, kc_sn, kc_sh, vc_sp, vc_sn, vc_sh;
+  int64_t window, sinks;               /* window 0: every earlier key is visible */
+  void* workspace; int64_t workspace_bytes;
+} LlcPagedAttentionParams;
+int llc_cuda_paged_attention(const LlcPagedAttentionParams* p, void* stream);
+/* Bytes of workspace that the call can use (it depends on shapes and types alone); 0 when it uses none. */
+int64_t llc_cuda_paged_attention_workspace(const LlcPagedAttentionParams* p);
+
 /* x [n, c, hw] (NCHW planes) -> out [n, hw, c_pad] (NHWC pixels), channels c..c_pad-1 written as
  * zeros.  The layout change the reference expresses as llh.transpose perms [0,2,3,1] around conv
  * (src/Dialect/LLH/Transforms/TransformLayout.cpp:141-198), with the channel padding the

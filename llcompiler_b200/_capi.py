@@ -38,6 +38,7 @@ def lib() -> ctypes.CDLL:
         _lib.llc_version.restype = c_char_p
         _lib.llc_compile.argtypes = [c_char_p, POINTER(LlcOptions), c_char_p, c_size_t]
         _lib.llc_run_pass.argtypes = [c_char_p, c_char_p, POINTER(LlcOptions), POINTER(c_char_p)]
+        _lib.llc_cuda_paged_attention_workspace.restype = c_int64
         _lib.llc_cuda_push_rows.argtypes = [ctypes.c_void_p, POINTER(ctypes.c_void_p), ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p]
     return _lib
 
@@ -137,10 +138,31 @@ class LlcEmbedNormParams(Structure):
                 ("dtype", c_int32)] + [(n, c_int64) for n in ("rows", "d", "vocab", "period", "add_s0", "add_s1")] + [("eps", c_float), ("bad_ids", c_void_p)]
 
 
+class LlcRotaryParams(Structure):
+    _fields_ = [("x", c_void_p), ("out", c_void_p), ("positions", c_void_p), ("inv_freq", c_void_p), ("dtype", c_int32), ("pos_dtype", c_int32)] + \
+               [(n, c_int64) for n in ("tokens", "heads", "d", "pairs", "x_st", "x_sh", "o_st", "o_sh", "pos_sa")] + \
+               [("axes", c_int32), ("interleaved", c_int32), ("sections", c_int32 * 4)]
+
+
+class LlcKvAppendParams(Structure):
+    _fields_ = [(n, c_void_p) for n in ("k", "v", "k_cache", "v_cache", "q", "q_out", "page_table", "q_start", "kv_len", "positions", "inv_freq", "bad_pages")] + \
+               [("dtype", c_int32), ("pos_dtype", c_int32)] + \
+               [(n, c_int64) for n in ("tokens", "batch", "heads", "kv_heads", "d", "pairs", "num_pages", "page_size", "table_width", "table_s0",
+                                       "q_st", "q_sh", "qo_st", "qo_sh", "k_st", "k_sh", "v_st", "v_sh", "kc_sp", "kc_sn", "kc_sh", "vc_sp", "vc_sn", "vc_sh", "pos_sa")] + \
+               [("axes", c_int32), ("interleaved", c_int32), ("sections", c_int32 * 4)]
+
+
+class LlcPagedAttentionParams(Structure):
+    _fields_ = [(n, c_void_p) for n in ("q", "k_cache", "v_cache", "out", "page_table", "q_start", "kv_len", "bad_pages")] + \
+               [("dtype", c_int32), ("scale", c_float)] + \
+               [(n, c_int64) for n in ("tokens", "batch", "heads", "kv_heads", "d", "max_q", "num_pages", "page_size", "table_width", "table_s0", "q_st", "q_sh", "o_st", "o_sh",
+                                       "kc_sp", "kc_sn", "kc_sh", "vc_sp", "vc_sn", "vc_sh", "window", "sinks")] + [("workspace", c_void_p), ("workspace_bytes", c_int64)]
+
+
 EXPORTED_SYMBOLS = [
     "llc_compile", "llc_run_pass", "llc_load", "llc_load_from", "llc_loaded_from_pool", "llc_num_inputs", "llc_num_outputs", "llc_num_symbols",
     "llc_output_shape", "llc_run", "llc_profile", "llc_status", "llc_last_launch_count", "llc_arena_bytes", "llc_free", "llc_last_error",
     "llc_version", "llc_cuda_gemm", "llc_cuda_conv2d", "llc_cuda_maxpool2d", "llc_cuda_reduce",
     "llc_cuda_softmax", "llc_cuda_layernorm", "llc_cuda_gather", "llc_cuda_eltwise", "llc_cuda_status", "llc_cuda_nchw_to_nhwc", "llc_cuda_gemm_static_scratch", "llc_cuda_attention", "llc_cuda_nchw_to_nhwc_wide",
-    "llc_cuda_push_rows", "llc_cuda_embed_norm",
+    "llc_cuda_push_rows", "llc_cuda_embed_norm", "llc_cuda_rotary", "llc_cuda_kv_append", "llc_cuda_paged_attention", "llc_cuda_paged_attention_workspace",
 ]

@@ -1,0 +1,141 @@
+// Attention of new tokens over a paged key / value cache: argument checks, the choice of kernel, and the kernel of plain
+// multiply-adds that takes every type, head size, page size and stride.
+#include "paged_attention.cuh"
+
+namespace llc {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kMaxD = 256;
+
+// One block per (token, head): the warps take the visible keys in turn, each with a running maximum and sum, lane l holding
+// elements l, l + 32, ... of the row, and meet in shared memory at the end.  out = sum_w o_w 2^(m_w - m) / sum_w l_w 2^(m_w - m).
+template <typename T>
+__global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedArgs p) {
+  __shared__ float sM[kWarps], sL[kWarps], sO[kWarps][kMaxD];
+  __shared__ int sSeq;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long t = blockIdx.x / p.heads;
+  const int h = (int)(blockIdx.x - t * p.heads);
+  if (warp == 0) {
+    // sequences that end at or before row t, 32 ends at a time
+    int c = 0;
+    for (int i = lane; i < p.batch; i += 32) c += p.qStart[i + 1] <= t;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0) sSeq = c;
+  }
+  __syncthreads();
+  const int b = sSeq;
+  if (b >= p.batch || t < p.qStart[b]) return;         // a row of nobody
+  const Sequence s = sequenceOf(p, b);
+  if (s.n == 0) return;
+  const long long pos = s.len - s.n + (t - s.begin);
+  const long long lo = pos + 1 - p.window > 0 ? pos + 1 - p.window : 0, first = p.sinks < lo ? p.sinks : lo;
+  const long long keys = pos < 0 ? 0 : first + (pos + 1 - lo);
+  const int g = h / p.group;
+  constexpr int kPer = kMaxD / 32;
+  float q[kPer], o[kPer], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = lane + 32 * i;
+    q[i] = e < p.d ? loadAs(p.q, t * p.qSt + h * p.qSh + e, p.dtype) * p.scaleLog2 : 0.f;
+    o[i] = 0.f;
+  }
+  for (long long idx = warp; idx < keys; idx += kWarps) {
+    const long long j = idx < first ? idx : idx - first + lo;
+    const long long page = pageOf(p, b, j / p.pageSize), slot = j % p.pageSize;
+    if (page < 0 && lane == 0 && p.badPages) atomicAdd(p.badPages, 1);
+    const T* k = reinterpret_cast<const T*>(p.k) + page * p.kcSp + slot * p.kcSn + g * p.kcSh;
+    const T* v = reinterpret_cast<const T*>(p.v) + page * p.vcSp + slot * p.vcSn + g * p.vcSh;
+    float dot = 0.f, vv[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int e = lane + 32 * i;
+      const bool in = page >= 0 && e < p.d;
+      dot = fmaf(in ? (float)k[e] : 0.f, q[i], dot);
+      vv[i] = in ? (float)v[e] : 0.f;
+    }
+    dot = warpSum(dot);
+    const float mNew = fmaxf(m, dot);
+    const float base = mNew == -INFINITY ? 0.f : mNew;
+    const float keep = exp2f(m - base), w = exp2f(dot - base);
+    m = mNew;
+    l = l * keep + w;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) o[i] = fmaf(w, vv[i], o[i] * keep);
+  }
+  if (lane == 0) { sM[warp] = m; sL[warp] = l; }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) sO[warp][lane + 32 * i] = o[i];
+  __syncthreads();
+  float top = sM[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sM[w]);
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, f[kWarps];
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) { f[w] = exp2f(sM[w] - base); sum += sL[w] * f[w]; }
+  for (int e = threadIdx.x; e < p.d; e += kWarps * 32) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) x += sO[w][e] * f[w];
+    storeAs(p.out, t * p.oSt + h * p.oSh + e, p.dtype, sum == 0.f ? 0.f : x / sum);
+  }
+}
+
+int pagedRows(const PagedArgs& a, cudaStream_t st) {
+  const long long grid = a.tokens * a.heads;
+  if (grid > 0x7FFFFFFFLL) return setError(LLC_ERR_UNSUPPORTED, "llc argument: paged_attention too many rows");
+  if (a.dtype == LLC_FLOAT32) paged_rows_kernel<float><<<(unsigned)grid, kWarps * 32, 0, st>>>(a);
+  else if (a.dtype == LLC_BFLOAT16) paged_rows_kernel<__nv_bfloat16><<<(unsigned)grid, kWarps * 32, 0, st>>>(a);
+  else paged_rows_kernel<__half><<<(unsigned)grid, kWarps * 32, 0, st>>>(a);
+  LLC_LAUNCH_CHECK("paged_rows_kernel");
+  return LLC_OK;
+}
+
+int checkAndFill(const LlcPagedAttentionParams* p, PagedArgs* a) {
+  if (!p) return setError(LLC_ERR_ARGUMENT, "llc argument: paged_attention null parameter block");
+  if (p->tokens < 0 || p->batch < 0 || p->heads < 1 || p->kv_heads < 1 || p->d < 1 || p->max_q < 0 || p->num_pages < 0 || p->page_size < 1 || p->table_width < 0)
+    return setError(LLC_ERR_ARGUMENT, "llc argument: paged_attention extents");
+  if (p->heads % p->kv_heads) return setError(LLC_ERR_ARGUMENT, "llc argument: paged_attention heads must be a multiple of kv_heads");
+  if (p->window < 0 || p->sinks < 0) return setError(LLC_ERR_ARGUMENT, "llc argument: paged_attention negative window or sinks");
+  if (p->dtype != LLC_FLOAT32 && p->dtype != LLC_BFLOAT16 && p->dtype != LLC_FLOAT16)
+    return setError(LLC_ERR_UNSUPPORTED, "llc argument: paged_attention tensors must be f32, bf16 or f16");
+  if (p->d > kMaxD) return setError(LLC_ERR_UNSUPPORTED, "llc argument: paged_attention head size above 256");
+  if (p->tokens > 0x7FFFFFFFLL || p->batch > (1 << 20) || p->heads > 65536 || p->num_pages > 0x7FFFFFFFLL || p->page_size > (1 << 20) || p->table_width > 0x7FFFFFFFLL)
+    return setError(LLC_ERR_UNSUPPORTED, "llc argument: paged_attention too large");
+  if (p->table_width * p->page_size > 0x7FFFFF00LL) return setError(LLC_ERR_UNSUPPORTED, "llc argument: paged_attention table reaches past 2^31 slots");
+  a->q = p->q; a->k = p->k_cache; a->v = p->v_cache; a->out = p->out;
+  a->table = p->page_table; a->qStart = p->q_start; a->kvLen = p->kv_len; a->badPages = p->bad_pages;
+  a->qSt = p->q_st; a->qSh = p->q_sh; a->oSt = p->o_st; a->oSh = p->o_sh;
+  a->kcSp = p->kc_sp; a->kcSn = p->kc_sn; a->kcSh = p->kc_sh; a->vcSp = p->vc_sp; a->vcSn = p->vc_sn; a->vcSh = p->vc_sh;
+  a->tableS0 = p->table_s0; a->tokens = p->tokens; a->numPages = p->num_pages; a->pageSize = p->page_size;
+  a->reach = p->table_width * p->page_size;
+  a->maxQ = p->max_q < p->tokens ? p->max_q : p->tokens;
+  a->window = p->window > 0 && p->window < a->reach ? p->window : a->reach + 1;
+  a->sinks = p->sinks < a->reach ? p->sinks : a->reach;
+  a->batch = (int)p->batch; a->heads = (int)p->heads; a->kvHeads = (int)p->kv_heads; a->group = (int)(p->heads / p->kv_heads);
+  a->d = (int)p->d; a->dtype = p->dtype;
+  a->scaleLog2 = p->scale * 1.4426950408889634f;
+  return LLC_OK;
+}
+
+}  // namespace
+}  // namespace llc
+
+using namespace llc;
+
+extern "C" int64_t llc_cuda_paged_attention_workspace(const LlcPagedAttentionParams* p) {
+  PagedArgs a{};
+  if (checkAndFill(p, &a) != LLC_OK) return 0;
+  return 0;
+}
+
+extern "C" int llc_cuda_paged_attention(const LlcPagedAttentionParams* p, void* stream) {
+  PagedArgs a{};
+  if (int rc = checkAndFill(p, &a)) return rc;
+  if (a.tokens == 0 || a.batch == 0 || a.maxQ == 0) return LLC_OK;
+  if (!p->q || !p->out || !p->q_start || !p->kv_len || (a.reach > 0 && !p->page_table) || (p->num_pages > 0 && (!p->k_cache || !p->v_cache)))
+    return setError(LLC_ERR_ARGUMENT, "llc argument: paged_attention null operand");
+  return pagedRows(a, (cudaStream_t)stream);
+}

@@ -7,11 +7,13 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
+#include <array>
 #include <cstring>
 #include <stdexcept>
 #include <string>
 #include <vector>
 
+#include "llc_cuda.h"
 #include "llc_runtime.h"
 
 namespace py = pybind11;
@@ -162,6 +164,60 @@ struct Execution {
   int64_t arena_bytes() const { need(); return llc_arena_bytes(exec); }
 };
 
+// Operators of the kernel library that a serving loop calls on device tensors directly, without a compiled plan: addresses,
+// extents and strides in, one launch on `stream` out.  The Python side (executor/paged.py) looks after shapes and devices.
+template <size_t N> using Ints = std::array<int64_t, N>;
+const void* at(int64_t p) { return reinterpret_cast<const void*>(static_cast<uintptr_t>(p)); }
+void* to(int64_t p) { return reinterpret_cast<void*>(static_cast<uintptr_t>(p)); }
+
+// pointers: x, out, positions, inv_freq; sizes: tokens, heads, d, pairs; strides: x_st, x_sh, o_st, o_sh, pos_sa
+void rotary(const Ints<4>& ptr, int dtype, int pos_dtype, const Ints<4>& n, const Ints<5>& s, int axes, const Ints<4>& sections, bool interleaved, uintptr_t stream) {
+  LlcRotaryParams p{};
+  p.x = at(ptr[0]); p.out = to(ptr[1]); p.positions = at(ptr[2]); p.inv_freq = static_cast<const double*>(at(ptr[3]));
+  p.dtype = dtype; p.pos_dtype = pos_dtype; p.tokens = n[0]; p.heads = n[1]; p.d = n[2]; p.pairs = n[3];
+  p.x_st = s[0]; p.x_sh = s[1]; p.o_st = s[2]; p.o_sh = s[3]; p.pos_sa = s[4]; p.axes = axes; p.interleaved = interleaved;
+  for (int i = 0; i < 4; ++i) p.sections[i] = (int32_t)sections[i];
+  check(llc_cuda_rotary(&p, reinterpret_cast<void*>(stream)));
+}
+
+// pointers: k, v, k_cache, v_cache, q, q_out, page_table, q_start, kv_len, positions, inv_freq, bad_pages; sizes: tokens, batch, heads, kv_heads, d,
+// pairs, num_pages, page_size, table_width, table_s0; strides: q_st, q_sh, qo_st, qo_sh, k_st, k_sh, v_st, v_sh, then page, slot and head of each cache, pos_sa
+void kvAppend(const Ints<12>& ptr, int dtype, int pos_dtype, const Ints<10>& n, const Ints<15>& s, int axes, const Ints<4>& sections, bool interleaved, uintptr_t stream) {
+  LlcKvAppendParams p{};
+  p.k = at(ptr[0]); p.v = at(ptr[1]); p.k_cache = to(ptr[2]); p.v_cache = to(ptr[3]); p.q = at(ptr[4]); p.q_out = to(ptr[5]);
+  p.page_table = static_cast<const int32_t*>(at(ptr[6])); p.q_start = static_cast<const int32_t*>(at(ptr[7])); p.kv_len = static_cast<const int32_t*>(at(ptr[8]));
+  p.positions = at(ptr[9]); p.inv_freq = static_cast<const double*>(at(ptr[10])); p.bad_pages = static_cast<int32_t*>(to(ptr[11]));
+  p.dtype = dtype; p.pos_dtype = pos_dtype;
+  p.tokens = n[0]; p.batch = n[1]; p.heads = n[2]; p.kv_heads = n[3]; p.d = n[4]; p.pairs = n[5]; p.num_pages = n[6]; p.page_size = n[7]; p.table_width = n[8]; p.table_s0 = n[9];
+  p.q_st = s[0]; p.q_sh = s[1]; p.qo_st = s[2]; p.qo_sh = s[3]; p.k_st = s[4]; p.k_sh = s[5]; p.v_st = s[6]; p.v_sh = s[7];
+  p.kc_sp = s[8]; p.kc_sn = s[9]; p.kc_sh = s[10]; p.vc_sp = s[11]; p.vc_sn = s[12]; p.vc_sh = s[13]; p.pos_sa = s[14];
+  p.axes = axes; p.interleaved = interleaved;
+  for (int i = 0; i < 4; ++i) p.sections[i] = (int32_t)sections[i];
+  check(llc_cuda_kv_append(&p, reinterpret_cast<void*>(stream)));
+}
+
+// pointers: q, k_cache, v_cache, out, page_table, q_start, kv_len, bad_pages; sizes: tokens, batch, heads, kv_heads, d, max_q, num_pages, page_size, table_width,
+// table_s0, window, sinks; strides: q_st, q_sh, o_st, o_sh, then page, slot and head of each cache
+LlcPagedAttentionParams pagedParams(const Ints<8>& ptr, int dtype, float scale, const Ints<12>& n, const Ints<10>& s) {
+  LlcPagedAttentionParams p{};
+  p.q = at(ptr[0]); p.k_cache = at(ptr[1]); p.v_cache = at(ptr[2]); p.out = to(ptr[3]);
+  p.page_table = static_cast<const int32_t*>(at(ptr[4])); p.q_start = static_cast<const int32_t*>(at(ptr[5])); p.kv_len = static_cast<const int32_t*>(at(ptr[6]));
+  p.bad_pages = static_cast<int32_t*>(to(ptr[7])); p.dtype = dtype; p.scale = scale;
+  p.tokens = n[0]; p.batch = n[1]; p.heads = n[2]; p.kv_heads = n[3]; p.d = n[4]; p.max_q = n[5]; p.num_pages = n[6]; p.page_size = n[7]; p.table_width = n[8];
+  p.table_s0 = n[9]; p.window = n[10]; p.sinks = n[11];
+  p.q_st = s[0]; p.q_sh = s[1]; p.o_st = s[2]; p.o_sh = s[3]; p.kc_sp = s[4]; p.kc_sn = s[5]; p.kc_sh = s[6]; p.vc_sp = s[7]; p.vc_sn = s[8]; p.vc_sh = s[9];
+  return p;
+}
+int64_t pagedWorkspace(const Ints<8>& ptr, int dtype, float scale, const Ints<12>& n, const Ints<10>& s) {
+  LlcPagedAttentionParams p = pagedParams(ptr, dtype, scale, n, s);
+  return llc_cuda_paged_attention_workspace(&p);
+}
+void pagedAttention(const Ints<8>& ptr, int dtype, float scale, const Ints<12>& n, const Ints<10>& s, uintptr_t workspace, int64_t bytes, uintptr_t stream) {
+  LlcPagedAttentionParams p = pagedParams(ptr, dtype, scale, n, s);
+  p.workspace = reinterpret_cast<void*>(workspace); p.workspace_bytes = bytes;
+  check(llc_cuda_paged_attention(&p, reinterpret_cast<void*>(stream)));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(llcompiler_, m) {
@@ -213,5 +269,10 @@ PYBIND11_MODULE(llcompiler_, m) {
       .def("status", &Execution::status)
       .def("num_inputs", &Execution::num_inputs).def("num_outputs", &Execution::num_outputs).def("num_symbols", &Execution::num_symbols)
       .def("last_launch_count", &Execution::last_launch_count).def("arena_bytes", &Execution::arena_bytes);
+  auto ops = m.def_submodule("ops");
+  ops.def("rotary", &rotary);
+  ops.def("kv_append", &kvAppend);
+  ops.def("paged_attention_workspace", &pagedWorkspace);
+  ops.def("paged_attention", &pagedAttention);
   m.def("version", []() { return std::string(llc_version()); });
 }

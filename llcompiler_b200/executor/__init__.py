@@ -1,11 +1,15 @@
 from .sharded import BatchShardedRunner, gather_batch, shard_bounds
 
-__all__ = ["ExecutionEngine", "Torch_ExecutionEngine", "BatchShardedRunner", "gather_batch", "shard_bounds"]
+__all__ = ["ExecutionEngine", "Torch_ExecutionEngine", "BatchShardedRunner", "gather_batch", "shard_bounds", "rotary",
+           "kv_append", "paged_attention"]
 
 
 def __getattr__(name):
-    # the engines need the llcompiler_ extension (and a GPU); the sharding helpers do not
+    # the engines and the decoder operators need the llcompiler_ extension (and a GPU); the sharding helpers do not
     if name in ("ExecutionEngine", "Torch_ExecutionEngine", "TORCH_DTYPE_TO_TYPE"):
         from . import engine
         return getattr(engine, name)
+    if name in ("rotary", "kv_append", "paged_attention"):
+        from . import paged
+        return getattr(paged, name)
     raise AttributeError(name)
