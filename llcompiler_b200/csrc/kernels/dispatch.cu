@@ -11,6 +11,7 @@ bool tcConvSupported(const LlcConvParams* p);
 int tcConv(const LlcConvParams* p, cudaStream_t st);
 int tcStatus();
 int attnStatus();
+int pagedDecodeStatus();
 }  // namespace llc
 
 using namespace llc;
@@ -29,8 +30,8 @@ extern "C" int llc_cuda_gemm(const LlcGemmParams* p, void* stream) {
 }
 
 extern "C" int llc_cuda_status(void) {
-  const int a = tcStatus(), b = attnStatus();
-  return a ? a : b;
+  const int a = tcStatus(), b = attnStatus(), c = pagedDecodeStatus();
+  return a ? a : b ? b : c;
 }
 
 extern "C" int llc_cuda_conv2d(const LlcConvParams* p, void* stream) {

@@ -3,6 +3,9 @@
 #include "paged_attention.cuh"
 
 namespace llc {
+long long pagedDecodeWorkspace(const PagedArgs& p, bool wide);
+int pagedDecode(const PagedArgs& p, bool wide, void* workspace, long long bytes, cudaStream_t st);
+
 namespace {
 
 constexpr int kWarps = 8;
@@ -11,7 +14,7 @@ constexpr int kMaxD = 256;
 // One block per (token, head): the warps take the visible keys in turn, each with a running maximum and sum, lane l holding
 // elements l, l + 32, ... of the row, and meet in shared memory at the end.  out = sum_w o_w 2^(m_w - m) / sum_w l_w 2^(m_w - m).
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedArgs p) {
+__global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedArgs p, int doneRows) {
   __shared__ float sM[kWarps], sL[kWarps], sO[kWarps][kMaxD];
   __shared__ int sSeq;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -28,7 +31,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedArgs
   const int b = sSeq;
   if (b >= p.batch || t < p.qStart[b]) return;         // a row of nobody
   const Sequence s = sequenceOf(p, b);
-  if (s.n == 0) return;
+  if (s.n == 0 || s.n * p.group <= doneRows) return;   // another kernel's
   const long long pos = s.len - s.n + (t - s.begin);
   const long long lo = pos + 1 - p.window > 0 ? pos + 1 - p.window : 0, first = p.sinks < lo ? p.sinks : lo;
   const long long keys = pos < 0 ? 0 : first + (pos + 1 - lo);
@@ -83,12 +86,13 @@ __global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedArgs
   }
 }
 
-int pagedRows(const PagedArgs& a, cudaStream_t st) {
+// doneRows: sequences of at most that many rows (new tokens x query heads of a key head) are left alone.
+int pagedRows(const PagedArgs& a, int doneRows, cudaStream_t st) {
   const long long grid = a.tokens * a.heads;
   if (grid > 0x7FFFFFFFLL) return setError(LLC_ERR_UNSUPPORTED, "llc argument: paged_attention too many rows");
-  if (a.dtype == LLC_FLOAT32) paged_rows_kernel<float><<<(unsigned)grid, kWarps * 32, 0, st>>>(a);
-  else if (a.dtype == LLC_BFLOAT16) paged_rows_kernel<__nv_bfloat16><<<(unsigned)grid, kWarps * 32, 0, st>>>(a);
-  else paged_rows_kernel<__half><<<(unsigned)grid, kWarps * 32, 0, st>>>(a);
+  if (a.dtype == LLC_FLOAT32) paged_rows_kernel<float><<<(unsigned)grid, kWarps * 32, 0, st>>>(a, doneRows);
+  else if (a.dtype == LLC_BFLOAT16) paged_rows_kernel<__nv_bfloat16><<<(unsigned)grid, kWarps * 32, 0, st>>>(a, doneRows);
+  else paged_rows_kernel<__half><<<(unsigned)grid, kWarps * 32, 0, st>>>(a, doneRows);
   LLC_LAUNCH_CHECK("paged_rows_kernel");
   return LLC_OK;
 }
@@ -120,6 +124,24 @@ int checkAndFill(const LlcPagedAttentionParams* p, PagedArgs* a) {
   return LLC_OK;
 }
 
+// What the tensor-core kernels take: the types, head sizes and pages they have tiles for, and 16-byte steps everywhere.
+bool tensorTypes(const PagedArgs& a) {
+  bool ok = a.dtype != LLC_FLOAT32 && (a.d == 64 || a.d == 128) && a.pageSize >= 16 && (a.pageSize & (a.pageSize - 1)) == 0 && a.numPages > 0 && a.reach > 0 &&
+            (long long)a.batch * a.kvHeads <= 0x7FFFFFFFLL;
+  for (long long s : {a.qSt, a.qSh, a.oSt, a.oSh}) ok = ok && s % 8 == 0;
+  for (long long s : {a.kcSp, a.kcSn, a.kcSh, a.vcSp, a.vcSn, a.vcSh}) ok = ok && s % 8 == 0 && s > 0 && s < (1LL << 38);
+  for (const void* x : {a.q, a.k, a.v, (const void*)a.out}) ok = ok && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  return ok;
+}
+
+// Rows of a sequence up to which the decode kernel takes it.  A call whose sequences all have at most 32 rows runs there alone; beside
+// longer chunks it takes the sequences of single tokens (16 rows, which leave two CTAs on an SM, or 32 for large groups).
+int decodeRows(const PagedArgs& a) {
+  const long long rows = a.maxQ * a.group;
+  if (rows <= 32) return rows <= 16 ? 16 : 32;
+  return a.group <= 16 ? 16 : a.group <= 32 ? 32 : 0;
+}
+
 }  // namespace
 }  // namespace llc
 
@@ -127,8 +149,9 @@ using namespace llc;
 
 extern "C" int64_t llc_cuda_paged_attention_workspace(const LlcPagedAttentionParams* p) {
   PagedArgs a{};
-  if (checkAndFill(p, &a) != LLC_OK) return 0;
-  return 0;
+  if (checkAndFill(p, &a) != LLC_OK || !tensorTypes(a) || a.tokens == 0 || a.batch == 0 || a.maxQ == 0) return 0;
+  const int few = decodeRows(a);
+  return few ? pagedDecodeWorkspace(a, few == 32) : 0;
 }
 
 extern "C" int llc_cuda_paged_attention(const LlcPagedAttentionParams* p, void* stream) {
@@ -137,5 +160,11 @@ extern "C" int llc_cuda_paged_attention(const LlcPagedAttentionParams* p, void* 
   if (a.tokens == 0 || a.batch == 0 || a.maxQ == 0) return LLC_OK;
   if (!p->q || !p->out || !p->q_start || !p->kv_len || (a.reach > 0 && !p->page_table) || (p->num_pages > 0 && (!p->k_cache || !p->v_cache)))
     return setError(LLC_ERR_ARGUMENT, "llc argument: paged_attention null operand");
-  return pagedRows(a, (cudaStream_t)stream);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (!tensorTypes(a)) return pagedRows(a, 0, st);
+  const int few = decodeRows(a);
+  if (few) {
+    if (int rc = pagedDecode(a, few == 32, p->workspace, p->workspace_bytes, st)) return rc;
+  }
+  return a.maxQ * a.group > few ? pagedRows(a, few, st) : LLC_OK;
 }
