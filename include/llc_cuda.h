@@ -83,7 +83,7 @@ typedef struct LlcAttentionParams {
 int llc_cuda_attention(const LlcAttentionParams* p, void* stream);
 
 /* Health word of the tensor-core kernels.  Their waits on memory barriers are bounded; a wait that
- * gives up records 1 (producer), 2 (issuer), 3 (operand split), 4 (epilogue), 5 (gather), 6 or 7 (attention), 8 or 9 (paged attention) and the launch's
+ * gives up records 1 (producer), 2 (issuer), 3 (operand split), 4 (epilogue), 5 (gather), 6 or 7 (attention), 8 to 12 (paged attention) and the launch's
  * result is then invalid.  Returns the recorded code (0 = healthy) and clears it; -1 if the device
  * cannot be read.  Synchronises the device.  No counterpart in the reference. */
 int llc_cuda_status(void);

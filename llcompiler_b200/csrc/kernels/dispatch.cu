@@ -12,6 +12,7 @@ int tcConv(const LlcConvParams* p, cudaStream_t st);
 int tcStatus();
 int attnStatus();
 int pagedDecodeStatus();
+int pagedChunkStatus();
 }  // namespace llc
 
 using namespace llc;
@@ -30,8 +31,8 @@ extern "C" int llc_cuda_gemm(const LlcGemmParams* p, void* stream) {
 }
 
 extern "C" int llc_cuda_status(void) {
-  const int a = tcStatus(), b = attnStatus(), c = pagedDecodeStatus();
-  return a ? a : b ? b : c;
+  const int a = tcStatus(), b = attnStatus(), c = pagedDecodeStatus(), d = pagedChunkStatus();
+  return a ? a : b ? b : c ? c : d;
 }
 
 extern "C" int llc_cuda_conv2d(const LlcConvParams* p, void* stream) {

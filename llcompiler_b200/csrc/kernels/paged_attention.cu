@@ -5,6 +5,8 @@
 namespace llc {
 long long pagedDecodeWorkspace(const PagedArgs& p, bool wide);
 int pagedDecode(const PagedArgs& p, bool wide, void* workspace, long long bytes, cudaStream_t st);
+long long pagedChunkWorkspace(const PagedArgs& p);
+int pagedChunk(const PagedArgs& p, int doneRows, void* workspace, long long bytes, cudaStream_t st);
 
 namespace {
 
@@ -14,7 +16,7 @@ constexpr int kMaxD = 256;
 // One block per (token, head): the warps take the visible keys in turn, each with a running maximum and sum, lane l holding
 // elements l, l + 32, ... of the row, and meet in shared memory at the end.  out = sum_w o_w 2^(m_w - m) / sum_w l_w 2^(m_w - m).
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedArgs p, int doneRows) {
+__global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedArgs p) {
   __shared__ float sM[kWarps], sL[kWarps], sO[kWarps][kMaxD];
   __shared__ int sSeq;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -31,7 +33,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedArgs
   const int b = sSeq;
   if (b >= p.batch || t < p.qStart[b]) return;         // a row of nobody
   const Sequence s = sequenceOf(p, b);
-  if (s.n == 0 || s.n * p.group <= doneRows) return;   // another kernel's
+  if (s.n == 0) return;
   const long long pos = s.len - s.n + (t - s.begin);
   const long long lo = pos + 1 - p.window > 0 ? pos + 1 - p.window : 0, first = p.sinks < lo ? p.sinks : lo;
   const long long keys = pos < 0 ? 0 : first + (pos + 1 - lo);
@@ -86,13 +88,12 @@ __global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedArgs
   }
 }
 
-// doneRows: sequences of at most that many rows (new tokens x query heads of a key head) are left alone.
-int pagedRows(const PagedArgs& a, int doneRows, cudaStream_t st) {
+int pagedRows(const PagedArgs& a, cudaStream_t st) {
   const long long grid = a.tokens * a.heads;
   if (grid > 0x7FFFFFFFLL) return setError(LLC_ERR_UNSUPPORTED, "llc argument: paged_attention too many rows");
-  if (a.dtype == LLC_FLOAT32) paged_rows_kernel<float><<<(unsigned)grid, kWarps * 32, 0, st>>>(a, doneRows);
-  else if (a.dtype == LLC_BFLOAT16) paged_rows_kernel<__nv_bfloat16><<<(unsigned)grid, kWarps * 32, 0, st>>>(a, doneRows);
-  else paged_rows_kernel<__half><<<(unsigned)grid, kWarps * 32, 0, st>>>(a, doneRows);
+  if (a.dtype == LLC_FLOAT32) paged_rows_kernel<float><<<(unsigned)grid, kWarps * 32, 0, st>>>(a);
+  else if (a.dtype == LLC_BFLOAT16) paged_rows_kernel<__nv_bfloat16><<<(unsigned)grid, kWarps * 32, 0, st>>>(a);
+  else paged_rows_kernel<__half><<<(unsigned)grid, kWarps * 32, 0, st>>>(a);
   LLC_LAUNCH_CHECK("paged_rows_kernel");
   return LLC_OK;
 }
@@ -150,8 +151,10 @@ using namespace llc;
 extern "C" int64_t llc_cuda_paged_attention_workspace(const LlcPagedAttentionParams* p) {
   PagedArgs a{};
   if (checkAndFill(p, &a) != LLC_OK || !tensorTypes(a) || a.tokens == 0 || a.batch == 0 || a.maxQ == 0) return 0;
+  // the two kernels of a mixed batch run one after the other and share it
   const int few = decodeRows(a);
-  return few ? pagedDecodeWorkspace(a, few == 32) : 0;
+  const int64_t d = few ? pagedDecodeWorkspace(a, few == 32) : 0, c = a.maxQ * a.group > few ? pagedChunkWorkspace(a) : 0;
+  return d > c ? d : c;
 }
 
 extern "C" int llc_cuda_paged_attention(const LlcPagedAttentionParams* p, void* stream) {
@@ -161,10 +164,10 @@ extern "C" int llc_cuda_paged_attention(const LlcPagedAttentionParams* p, void* 
   if (!p->q || !p->out || !p->q_start || !p->kv_len || (a.reach > 0 && !p->page_table) || (p->num_pages > 0 && (!p->k_cache || !p->v_cache)))
     return setError(LLC_ERR_ARGUMENT, "llc argument: paged_attention null operand");
   const cudaStream_t st = (cudaStream_t)stream;
-  if (!tensorTypes(a)) return pagedRows(a, 0, st);
+  if (!tensorTypes(a)) return pagedRows(a, st);
   const int few = decodeRows(a);
   if (few) {
     if (int rc = pagedDecode(a, few == 32, p->workspace, p->workspace_bytes, st)) return rc;
   }
-  return a.maxQ * a.group > few ? pagedRows(a, few, st) : LLC_OK;
+  return a.maxQ * a.group > few ? pagedChunk(a, few, p->workspace, p->workspace_bytes, st) : LLC_OK;
 }

@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace llc {
@@ -35,6 +37,41 @@ __device__ __forceinline__ long long pageOf(const PagedArgs& p, int b, long long
   const long long page = p.table[b * p.tableS0 + index];
   return page >= 0 && page < p.numPages ? page : -1;
 }
+
+// The keys that tokens at places first .. last of a sequence of len keys see, some of them at least: [0, sinkEnd) and [lo, hi).
+struct Seen { long long sinkEnd, lo, hi; };
+__device__ __forceinline__ Seen seenBy(const PagedArgs& p, long long first, long long last) {
+  Seen s;
+  s.hi = last + 1 > 0 ? last + 1 : 0;
+  s.lo = first + 1 - p.window > 0 ? first + 1 - p.window : 0;
+  if (s.lo > s.hi) s.lo = s.hi;
+  s.sinkEnd = p.sinks < s.lo ? p.sinks : s.lo;
+  return s;
+}
+// The same in blocks of keys: `sink` blocks from the start, then the blocks from `first` on, `count` in all.
+struct Blocks { int sink, first, count; };
+__device__ __forceinline__ Blocks blocksOf(const Seen& s, int keys) {
+  Blocks b;
+  b.first = (int)(s.lo / keys);
+  b.sink = (int)((s.sinkEnd + keys - 1) / keys);
+  if (b.sink > b.first) b.sink = b.first;
+  b.count = b.sink + (int)((s.hi + keys - 1) / keys) - b.first;
+  return b;
+}
+__device__ __forceinline__ long long keyOf(const Blocks& b, long long unit, int keys) { return (unit < b.sink ? unit : unit - b.sink + b.first) * keys; }
+
+// Two numbers rounded to T, and whether one of two packed numbers is NaN or infinite.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) { __nv_bfloat162 v = __floats2bfloat162_rn(x, y); return *reinterpret_cast<uint32_t*>(&v); }
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) { __half2 v = __floats2half2_rn(x, y); return *reinterpret_cast<uint32_t*>(&v); }
+template <typename T> __device__ __forceinline__ bool notFinite(uint32_t x) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (x & e) == e || (x & (e << 16)) == (e << 16);
+}
+// Weights are rounded to the tensors' type for the second product.  f16 weights are kept 2^7 times larger, so that a weight loses
+// bits to f16's subnormals only below 2^-21 of the largest (2^7 x 2^8 of lag stays below 65504).
+template <typename T> constexpr float weightShift() { return std::is_same<T, __half>::value ? 7.f : 0.f; }
+constexpr float kRescaleStep = 8.f;    // the running maximum follows in steps larger than 2^8 only: the weights stay below 2^8
 
 __device__ __forceinline__ float exp2Fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 

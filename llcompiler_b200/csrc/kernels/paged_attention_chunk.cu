@@ -1,0 +1,578 @@
+// Paged attention for chunks of new tokens, on the 5th-generation tensor cores.
+// Mathematics: as in the decode kernel, out = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m) with a running m.  The rows of a tile are
+// (token, query head) pairs of one key head, token-major, so that all query heads of a group read the keys once and a tile's rows
+// differ little in what they see.
+// A CTA takes two tiles of 128 rows and walks the blocks of 128 keys that either sees:
+//   8 softmax warps   four a tile, one thread a row: the row's 128 scores come out of tensor memory into registers once; maximum,
+//                     2^x, sum, weights back into tensor memory as 16-bit numbers over the scores' own columns, from where the
+//                     second product takes them as its A operand (they never cross shared memory)
+//   loader warp       one lane a page box: TMA loads of K and V blocks into a ring of slots
+//   issuer warp       S_A, S_B, then for every block: O_A += P_A V, S_A of the next block, O_B += P_B V, S_B of the next block, so that
+//                     one tile's softmax runs under the other tile's products
+// Tensor memory: S_A, S_B (128 columns each), O_A, O_B (d columns each).  The issuer's products run in the order of issue, so the next
+// S_A may overwrite P_A as soon as O_A += P_A V has been issued.
+// Bound: at d = 128 a block of two tiles costs 2048 cycles of products and as many of exponentials (16 a cycle and SM).
+#include "paged_attention.cuh"
+#include "tc_common.cuh"
+#include "tensor_map.h"
+
+namespace llc {
+__device__ int g_pagedChunkStatus = 0;    // non-zero after a bounded wait gave up: 10 loader, 11 issuer, 12 softmax
+
+namespace {
+using namespace tc;
+
+constexpr int kThreads = 384;             // 8 softmax warps, loader, issuer, two idle warps that fill the warpgroup
+constexpr int kTileRows = 128, kCtaRows = 256, kKeys = 128;
+constexpr int kMaxSplits = 32;
+
+template <int D> struct Config {
+  static constexpr int kAtom = 128 * 128;             // bytes of 128 rows x 64 elements
+  static constexpr int kTile = kAtom * (D / 64);      // Q of a tile, K or V of a block
+  static constexpr int kSlots = D == 128 ? 5 : 10;
+  static constexpr int kMisc = 1024;
+  static constexpr int kSmem = 2 * kTile + kSlots * kTile + kMisc;
+  static constexpr int kPart = kTileRows * (D + 2);   // floats of a tile's partial sums: O as [D / 4][128 rows] vectors, then m, then l
+  static_assert(kSmem + 1024 <= 228 * 1024, "one CTA an SM");
+};
+// Columns of tensor memory.
+constexpr uint32_t kColS = 0, kColO = 256;
+
+struct ChunkArgs {
+  PagedArgs p;
+  int doneRows;                // sequences of at most so many rows are the decode kernel's
+  int pageShift, boxRows, splits;
+  float scaleAbs, signQ;       // the scale's size; its sign goes into Q, so that the largest product is the largest score
+  int4* records;               // [tiles * key heads]: sequence (or -1) and first row of each pair of tiles
+  float* parts;                // [tiles * key heads][2][splits][kPart]
+};
+
+// What a tile's rows see, and which blocks it takes part in.
+struct Tile {
+  long long first, last;       // places of its first and last token
+  Seen seen;
+  __device__ bool active(long long j0) const { return j0 < seen.sinkEnd || (j0 < seen.hi && j0 + kKeys > seen.lo); }
+};
+__device__ __forceinline__ Tile tileOf(const PagedArgs& p, const Sequence& s, long long row0, long long rows) {
+  Tile t;
+  const long long rowEnd = row0 + kTileRows < rows ? row0 + kTileRows : rows;
+  if (row0 >= rowEnd) { t.first = 0; t.last = -1; t.seen = Seen{0, 0, 0}; return t; }
+  t.first = s.len - s.n + row0 / p.group;
+  t.last = s.len - s.n + (rowEnd - 1) / p.group;
+  t.seen = seenBy(p, t.first, t.last);
+  return t;
+}
+__device__ __forceinline__ long long tilesOf(const PagedArgs& p, int b, int doneRows) {
+  const long long rows = sequenceOf(p, b).n * p.group;
+  return rows <= doneRows ? 0 : (rows + kCtaRows - 1) / kCtaRows;
+}
+
+// A row's sum over its visible keys among the blocks [begin, end) by multiply-adds, one warp a row: lane l gets elements l, l + 32, ...
+// Taken for a row whose sum came out NaN or infinite though its weights are finite: some value in the blocks is, and the products
+// multiply every value of a block by every row's weights, those that are 0 because the row does not see the value too.
+template <typename T, int D>
+__device__ __noinline__ void sumRow(const ChunkArgs& a, int b, int h, long long qOff, long long pos, Blocks bl, int begin, int end, float base, float* o) {
+  const PagedArgs& p = a.p;
+  const int lane = threadIdx.x & 31;
+  float q[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) { q[i] = (float)reinterpret_cast<const T*>(p.q)[qOff + lane + 32 * i] * a.signQ; o[i] = 0.f; }
+  for (int u = begin; u < end; ++u) {
+    const long long j0 = keyOf(bl, u, kKeys);
+    for (long long j = j0; j < j0 + kKeys; ++j) {
+      if (!(j <= pos && (pos - j < p.window || j < p.sinks))) continue;
+      const long long page = pageOf(p, b, j >> a.pageShift), slot = j & ((1 << a.pageShift) - 1);
+      if (page < 0) continue;                         // its values are zeros
+      const T* k = reinterpret_cast<const T*>(p.k) + page * p.kcSp + slot * p.kcSn + h * p.kcSh;
+      const T* v = reinterpret_cast<const T*>(p.v) + page * p.vcSp + slot * p.vcSn + h * p.vcSh;
+      float dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) dot = fmaf((float)k[lane + 32 * i], q[i], dot);
+      const float w = exp2Fast(fmaf(warpSum(dot), a.scaleAbs, -base));
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) o[i] = fmaf(w, (float)v[lane + 32 * i], o[i]);
+    }
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const __grid_constant__ ChunkArgs a) {
+  using C = Config<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sQ = smem;                                 // [2] tiles; the outputs pass through here at the end
+  uint8_t* ring = smem + 2 * C::kTile;
+  uint8_t* misc = ring + C::kSlots * C::kTile;
+  uint64_t* kvFull = reinterpret_cast<uint64_t*>(misc);
+  uint64_t* kvEmpty = kvFull + C::kSlots;
+  uint64_t* sFull = kvEmpty + C::kSlots;              // [2] scores of a tile complete, and every product issued before them
+  uint64_t* pReady = sFull + 2;                       // [2] weights of a tile written, its sums rescaled
+  uint64_t* oFull = pReady + 2;                       // [2] all products of a tile complete
+  uint64_t* qReady = oFull + 2;                       // both tiles of Q written
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(misc + 256);
+  volatile int* abortWord = reinterpret_cast<volatile int*>(misc + 260);
+  int* sSeq = reinterpret_cast<int*>(misc + 264);
+  int* sTile = sSeq + 1;
+  long long* sScan = reinterpret_cast<long long*>(misc + 272);   // [12]
+  const PagedArgs& p = a.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // Which sequence and tiles: blockIdx.x = head and part of the keys, blockIdx.y = tile pair, counted from the last, which sees the
+  // most keys of its sequence.
+  const int h = blockIdx.x / a.splits, split = blockIdx.x - h * a.splits;
+  {
+    const int per = (p.batch + kThreads - 1) / kThreads, first = threadIdx.x * per;
+    long long mine = 0;
+    for (int i = first; i < first + per && i < p.batch; ++i) mine += tilesOf(p, i, a.doneRows);
+    long long run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += x; }
+    if (lane == 31) sScan[warp] = run;
+    if (threadIdx.x == 0) {
+      *sSeq = -1;
+      for (int i = 0; i < C::kSlots; ++i) { mbarInit(&kvFull[i], 1); mbarInit(&kvEmpty[i], 1); }
+      for (int t = 0; t < 2; ++t) { mbarInit(&sFull[t], 1); mbarInit(&pReady[t], 4); mbarInit(&oFull[t], 1); }
+      mbarInit(qReady, 8);
+      *abortWord = 0;
+      fenceBarrierInit();
+    }
+    __syncthreads();
+    long long before = run - mine, all = 0;
+    for (int w = 0; w < kThreads / 32; ++w) { if (w < warp) before += sScan[w]; all += sScan[w]; }
+    const long long want = all - 1 - (long long)blockIdx.y;
+    if (want >= before && want < before + mine) {
+      for (int i = first; i < first + per && i < p.batch; ++i) {
+        const long long c = tilesOf(p, i, a.doneRows);
+        if (want < before + c) { *sSeq = i; *sTile = (int)(want - before); break; }
+        before += c;
+      }
+    }
+    __syncthreads();
+  }
+  const int b = *sSeq;
+  const long long pair = (long long)blockIdx.y * p.kvHeads + h;
+  if (a.splits > 1 && split == 0 && threadIdx.x == 0) a.records[pair] = make_int4(b, b < 0 ? 0 : *sTile, 0, 0);
+  if (b < 0) return;                                  // fewer tiles than the grid has room for
+  if (smemAddr(smem) & 1023) {                        // the swizzled tiles need it; no static shared memory lies before them
+    if (threadIdx.x == 0) { atomicExch(&g_pagedChunkStatus, 10); if (a.splits > 1 && split == 0) a.records[pair] = make_int4(-1, 0, 0, 0); }
+    return;
+  }
+  const Sequence s = sequenceOf(p, b);
+  const long long rows = s.n * p.group, row0 = (long long)*sTile * kCtaRows;
+  const Tile tile0 = tileOf(p, s, row0, rows), tile1 = tileOf(p, s, row0 + kTileRows, rows);
+  const Seen seen = seenBy(p, tile0.first, tile1.last >= 0 ? tile1.last : tile0.last);
+  const Blocks bl = blocksOf(seen, kKeys);
+  const int share = (bl.count + a.splits - 1) / a.splits;
+  const int begin = share * split < bl.count ? share * split : bl.count, end = begin + share < bl.count ? begin + share : bl.count;
+
+  if (warp == 9) tmemAlloc(tmemSlot, 512);
+  tcFenceBefore();
+  __syncthreads();
+  tcFenceAfter();
+  const uint32_t tmem = *tmemSlot;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 8) {
+      // ---------------------------------------------------------------- loader: items K, V, K, V, ...
+      if (lane == 0) { prefetchTensorMap(&mapK); prefetchTensorMap(&mapV); }
+      const int boxes = kKeys / a.boxRows, loads = boxes * (D / 64), box = lane % boxes, half = lane / boxes;
+      bool ok = true;
+      uint32_t item = 0;
+      auto lookUp = [&](int u) -> long long {
+        const long long j = keyOf(bl, u, kKeys) + (long long)box * a.boxRows;
+        // a box that no row sees any key of is not looked up: it reads as zeros, as does one with a bad page number
+        if (lane >= loads || !(j < seen.sinkEnd || (j < seen.hi && j + a.boxRows > seen.lo))) return -1;
+        const long long page = pageOf(p, b, j >> a.pageShift);
+        if (page < 0 && half == 0 && p.badPages) atomicAdd(p.badPages, 1);
+        return page;
+      };
+      long long next = begin < end ? lookUp(begin) : -1;
+      for (int u = begin; u < end && ok; ++u) {
+        const long long page = next;
+        if (u + 1 < end) next = lookUp(u + 1);
+        const int slotIn = (int)((keyOf(bl, u, kKeys) + box * a.boxRows) & ((1 << a.pageShift) - 1));
+        for (int kv = 0; kv < 2 && ok; ++kv, ++item) {
+          const int st = item % C::kSlots;
+          if (item >= C::kSlots) ok = __all_sync(0xffffffffu, mbarWait(&kvEmpty[st], (item / C::kSlots - 1) & 1u, abortWord));
+          if (!ok) break;
+          if (lane == 0) mbarExpectTx(&kvFull[st], C::kTile);
+          __syncwarp();
+          if (lane < loads)
+            tmaLoad4d(ring + st * C::kTile + half * C::kAtom + box * a.boxRows * 128, kv ? &mapV : &mapK, &kvFull[st], half * 64, slotIn, h,
+                      page < 0 ? (int)p.numPages : (int)page);
+        }
+      }
+      if (!ok) {
+        if (lane == 0) atomicExch(&g_pagedChunkStatus, 10);
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);   // copies in flight land before the CTA gives its memory back
+      }
+    } else if (warp == 9 && lane == 0) {
+      // ---------------------------------------------------------------- issuer
+      constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
+      constexpr uint32_t idescS = instrDesc(fmt, kTileRows, kKeys, 0, 0), idescO = instrDesc(fmt, kTileRows, D, 0, 1);
+      bool ok = mbarWait(qReady, 0, abortWord);
+      uint32_t weights[2] = {0, 0};                   // blocks whose weights a tile's warps have handed over
+      bool started[2] = {false, false};
+      auto active = [&](int t, int u) { return (t ? tile1 : tile0).active(keyOf(bl, u, kKeys)); };
+      auto slotWait = [&](uint32_t item) { ok = ok && mbarWait(&kvFull[item % C::kSlots], (item / C::kSlots) & 1u, abortWord); };
+      auto issueS = [&](int t, uint32_t item) {
+        const uint32_t q = smemAddr(sQ + t * C::kTile), k = smemAddr(ring + (item % C::kSlots) * C::kTile);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+          mmaSS<false>(tmem + kColS + t * kKeys, smemDescKMajorSw128(q + (ks / 4) * C::kAtom) + 2 * (ks % 4), smemDescKMajorSw128(k + (ks / 4) * C::kAtom) + 2 * (ks % 4), idescS,
+                       ks > 0 ? 1u : 0u);
+        mmaCommit(&sFull[t]);
+      };
+      if (begin < end) {
+        slotWait(0);
+        tcFenceAfter();
+        for (int t = 0; t < 2; ++t) if (active(t, begin)) issueS(t, 0);
+        mmaCommit(&kvEmpty[0]);
+      }
+      for (int u = begin; u < end; ++u) {
+        const uint32_t vItem = 2 * (u - begin) + 1, kItem = vItem + 1;
+        bool haveV = false, haveK = false;
+        for (int t = 0; t < 2; ++t) {
+          if (active(t, u)) {
+            if (!haveV) { slotWait(vItem); haveV = true; }
+            ok = ok && mbarWait(&pReady[t], weights[t] & 1u, abortWord);
+            ++weights[t];
+            tcFenceAfter();
+            const uint32_t v = smemAddr(ring + (vItem % C::kSlots) * C::kTile);
+#pragma unroll
+            for (int ks = 0; ks < kKeys / 16; ++ks)
+              mmaTS(tmem + kColO + t * D, tmem + kColS + t * kKeys + 8 * ks, smemDescMnMajorSw128(v + ks * 16 * 128, C::kAtom), idescO, ks > 0 || started[t] ? 1u : 0u);
+            started[t] = true;
+          }
+          if (u + 1 < end && active(t, u + 1)) {
+            if (!haveK) { slotWait(kItem); haveK = true; tcFenceAfter(); }
+            issueS(t, kItem);
+          }
+        }
+        if (!haveV) slotWait(vItem);                  // a slot is given back only after its load has landed
+        mmaCommit(&kvEmpty[vItem % C::kSlots]);
+        if (u + 1 < end) {
+          if (!haveK) slotWait(kItem);
+          mmaCommit(&kvEmpty[kItem % C::kSlots]);
+        }
+      }
+      mmaCommit(&oFull[0]);
+      mmaCommit(&oFull[1]);
+      if (!ok) atomicExch(&g_pagedChunkStatus, 11);
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int t = warp >> 2, r = threadIdx.x & 127, q4 = warp & 3;
+    const Tile tile = t ? tile1 : tile0;
+    const long long row = row0 + t * kTileRows + r;
+    const bool live = row < rows;
+    const long long tok = (live ? row : rows - 1) / p.group;
+    const long long pos = s.len - s.n + tok;
+    const int head = h * p.group + (int)((live ? row : rows - 1) - tok * p.group);
+    const long long qOff = (s.begin + tok) * p.qSt + head * p.qSh, oOff = (s.begin + tok) * p.oSt + head * p.oSh;
+    uint8_t* tileQ = sQ + t * C::kTile;
+    constexpr int kChunks = D / 8;                    // 16-byte chunks of a row
+    constexpr int kRowsAtOnce = 32 / kChunks;         // rows that a warp's 16-byte accesses cover
+    // Q, a warp its own 32 rows: neighbouring lanes take neighbouring chunks of a row
+#pragma unroll 4
+    for (int i = 0; i < 32; i += kRowsAtOnce) {
+      const int src = i + lane / kChunks, c = lane % kChunks, rr = q4 * 32 + src;
+      const long long off = __shfl_sync(0xffffffffu, qOff, src);
+      const bool in = __shfl_sync(0xffffffffu, (int)live, src);
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (in) x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + off + c * 8);
+      if (a.signQ < 0.f) { x.x ^= 0x80008000u; x.y ^= 0x80008000u; x.z ^= 0x80008000u; x.w ^= 0x80008000u; }
+      *reinterpret_cast<uint4*>(tileQ + (c >> 3) * C::kAtom + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x;
+    }
+    fenceProxyAsync();
+    __syncwarp();
+    if (lane == 0) mbarArrive(qReady);
+
+    const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
+    const uint32_t colS = tmem + lanes + kColS + t * kKeys, colO = tmem + lanes + kColO + t * D;
+    constexpr float kShift = weightShift<T>();
+    float m = -INFINITY, l = 0.f;
+    uint32_t done = 0;                                // blocks of this tile so far
+    bool ok = true;
+    for (int u = begin; u < end; ++u) {
+      const long long j0 = keyOf(bl, u, kKeys);
+      if (!tile.active(j0)) continue;
+      if (ok && !mbarWait(&sFull[t], done & 1u, abortWord)) { ok = false; atomicExch(&g_pagedChunkStatus, 12); }
+      tcFenceAfter();
+      __syncwarp();
+      uint32_t x[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmemIssue32(colS + 32 * c, x[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmemWait32(x[c]);
+      // every row sees all keys: they lie before the tile's first token, and inside its last one's window or among the sinks
+      const bool whole = j0 + kKeys - 1 <= tile.first && (j0 > tile.last - p.window || j0 + kKeys <= p.sinks);
+      if (!whole) {
+        // visible columns: c <= hi and (c >= lo or c < sink)
+        const long long hi64 = pos - j0, lo64 = pos - p.window + 1 - j0, sink64 = p.sinks - j0;
+        const int hi = hi64 > kKeys ? kKeys : hi64 < -1 ? -1 : (int)hi64, lo = lo64 < 0 ? 0 : lo64 > kKeys ? kKeys : (int)lo64;
+        const int sink = sink64 < 0 ? 0 : sink64 > kKeys ? kKeys : (int)sink64;
+#pragma unroll
+        for (int c = 0; c < kKeys; ++c)
+          if (!(c <= hi && (c >= lo || c < sink))) x[c >> 5][c & 31] = 0xff800000u;   // -inf, whatever the score is
+      }
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = __uint_as_float(x[c][0]);
+#pragma unroll
+        for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(x[c][i]));
+      }
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scaleAbs;
+      float keep = 1.f;
+      if (top > m + kRescaleStep) { keep = exp2Fast(m - top); m = top; }
+      const float base = m == -INFINITY ? 0.f : m - kShift;
+      l *= keep;
+      if (done > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
+        // some row of the warp moved its maximum; the scores' barrier says that all products into O are complete
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          tmemLoad32x32(colO + c, o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] *= keep;
+          tmemStore32(colO + c, reinterpret_cast<uint32_t*>(o));
+          tmemStoreWait();
+        }
+      }
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int c = half * 64 + 2 * i;
+          float y0 = __uint_as_float(x[c >> 5][c & 31]), y1 = __uint_as_float(x[c >> 5][(c & 31) + 1]);
+          fma2(y0, y1, a.scaleAbs, a.scaleAbs, -base, -base);
+          y0 = exp2Fast(y0); y1 = exp2Fast(y1);
+          sum[(i & 1) * 2] += y0; sum[(i & 1) * 2 + 1] += y1;
+          w[i] = pack2<T>(y0, y1);
+        }
+        __syncwarp();
+        tmemStore32(colS + 32 * half, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmemStoreWait();
+      // Values of keys that no row sees may be NaN, and 0 x NaN is NaN: the tile that uses the block first zeroes them, thread r key r.
+      const bool clean = j0 + kKeys <= seen.sinkEnd || (j0 + kKeys <= seen.hi && (j0 >= seen.lo || seen.sinkEnd == seen.lo));
+      if (!clean && (t == 0 || !tile0.active(j0))) {
+        const uint32_t vItem = 2 * (u - begin) + 1;
+        if (ok && !mbarWait(&kvFull[vItem % C::kSlots], (vItem / C::kSlots) & 1u, abortWord)) { ok = false; atomicExch(&g_pagedChunkStatus, 12); }
+        const long long j = j0 + r;
+        if (!(j < seen.sinkEnd || (j >= seen.lo && j < seen.hi))) {
+#pragma unroll
+          for (int i = 0; i < kChunks; ++i) *reinterpret_cast<uint4*>(ring + (vItem % C::kSlots) * C::kTile + (i >> 3) * C::kAtom + r * 128 + ((i & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        fenceProxyAsync();
+      }
+      tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) mbarArrive(&pReady[t]);
+      ++done;
+    }
+    // ---------------------------------------------------------------- output
+    if (ok && !mbarWait(&oFull[t], 0, abortWord)) { ok = false; atomicExch(&g_pagedChunkStatus, 12); }
+    tcFenceAfter();
+    __syncwarp();
+    const float base = m == -INFINITY ? 0.f : m - kShift;
+    const bool cut = a.splits > 1;
+    float* part = a.parts + ((pair * 2 + t) * a.splits + split) * C::kPart;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    bool odd = false;
+    if (cut) {
+      part[kTileRows * D + r] = m;
+      part[kTileRows * (D + 1) + r] = l;
+    }
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+      float o[32];
+      if (done) tmemLoad32x32(colO + c, o);
+      else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) odd = odd || !(fabsf(o[i]) <= 3.402823466e38f);
+      if (cut) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<float4*>(part + ((long long)(c / 4 + i) * kTileRows + r) * 4) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int ch = c / 8 + i;
+          *reinterpret_cast<uint4*>(tileQ + (ch >> 3) * C::kAtom + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) =
+              make_uint4(pack2<T>(o[8 * i] * inv, o[8 * i + 1] * inv), pack2<T>(o[8 * i + 2] * inv, o[8 * i + 3] * inv), pack2<T>(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
+                         pack2<T>(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+        }
+      }
+    }
+    __syncwarp();
+    unsigned redo = __ballot_sync(0xffffffffu, odd && live && fabsf(l) <= 3.402823466e38f);
+    while (redo) {
+      const int src = __ffs(redo) - 1, rr = q4 * 32 + src;
+      redo &= redo - 1;
+      float o[D / 32];
+      sumRow<T, D>(a, b, h, __shfl_sync(0xffffffffu, qOff, src), __shfl_sync(0xffffffffu, pos, src), bl, begin, end, __shfl_sync(0xffffffffu, base, src), o);
+      const float f = __shfl_sync(0xffffffffu, inv, src);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const int e = lane + 32 * i;
+        if (cut) part[((long long)(e / 4) * kTileRows + rr) * 4 + (e & 3)] = o[i];
+        else {
+          T* dst = reinterpret_cast<T*>(tileQ + (e >> 6) * C::kAtom + rr * 128 + ((((e >> 3) & 7) ^ (rr & 7)) << 4)) + (e & 7);
+          if constexpr (std::is_same<T, __half>::value) *dst = __float2half_rn(o[i] * f);
+          else *dst = __float2bfloat16_rn(o[i] * f);
+        }
+      }
+    }
+    __syncwarp();
+    if (!cut) {
+#pragma unroll 4
+      for (int i = 0; i < 32; i += kRowsAtOnce) {
+        const int src = i + lane / kChunks, c = lane % kChunks, rr = q4 * 32 + src;
+        const long long off = __shfl_sync(0xffffffffu, oOff, src);
+        const bool in = __shfl_sync(0xffffffffu, (int)live, src);
+        const uint4 x = *reinterpret_cast<const uint4*>(tileQ + (c >> 3) * C::kAtom + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
+        if (in) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + off + c * 8) = x;
+      }
+    }
+  }
+  tcFenceBefore();
+  __syncthreads();
+  if (warp == 9) { tcFenceAfter(); tmemDealloc(tmem, 512); }
+}
+
+// Joins the parts of a tile: block = one tile of 128 rows, thread = one row and every other vector of four elements.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_chunk_join_kernel(const ChunkArgs a) {
+  using C = Config<D>;
+  __shared__ float sF[kMaxSplits][kTileRows];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const PagedArgs& p = a.p;
+  const long long pair = blockIdx.x >> 1;
+  const int t = blockIdx.x & 1, r = threadIdx.x & 127, side = threadIdx.x >> 7;
+  const int4 rec = a.records[pair];
+  if (rec.x < 0) return;
+  const Sequence s = sequenceOf(p, rec.x);
+  const long long rows = s.n * p.group, row = (long long)rec.y * kCtaRows + t * kTileRows + r;
+  const float* part = a.parts + (pair * 2 + t) * a.splits * C::kPart;
+  float top = -INFINITY, sum = 0.f;
+  for (int i = 0; i < a.splits; ++i) top = fmaxf(top, part[(long long)i * C::kPart + kTileRows * D + r]);
+  for (int i = 0; i < a.splits; ++i) {
+    const float m = part[(long long)i * C::kPart + kTileRows * D + r], l = part[(long long)i * C::kPart + kTileRows * (D + 1) + r];
+    const float f = m == -INFINITY ? 0.f : exp2Fast(m - top);
+    if (side == 0) sF[i][r] = f;
+    if (m != -INFINITY) sum += l * f;
+  }
+  __syncthreads();
+  if (row >= rows) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const long long tok = row / p.group;
+  const int head = (int)(pair % p.kvHeads) * p.group + (int)(row - tok * p.group);
+  T* out = reinterpret_cast<T*>(p.out) + (s.begin + tok) * p.oSt + head * p.oSh;
+  for (int c = side; c < D / 4; c += 2) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < a.splits; ++i) {
+      const float f = sF[i][r];
+      if (f != 0.f) {                                 // a part that saw nothing may hold anything
+        const float4 v = *reinterpret_cast<const float4*>(part + (long long)i * C::kPart + ((long long)c * kTileRows + r) * 4);
+        x.x = fmaf(v.x, f, x.x); x.y = fmaf(v.y, f, x.y); x.z = fmaf(v.z, f, x.z); x.w = fmaf(v.w, f, x.w);
+      }
+    }
+    *reinterpret_cast<uint2*>(out + 4 * c) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+  }
+}
+
+// Pairs of tiles that the grid has room for (a bound from what the host knows), and in how many parts the keys are taken: one where
+// the pairs alone fill the SMs, else as many as bring the grid to one CTA an SM, at least two blocks of keys each.
+struct Launch { long long tiles; int splits; };
+Launch launchOf(const PagedArgs& p) {
+  Launch l;
+  const long long each = (p.maxQ * p.group + kCtaRows - 1) / kCtaRows, most = p.tokens * p.group / kCtaRows + p.batch;
+  l.tiles = each * p.batch < most ? each * p.batch : most;
+  const long long ctas = l.tiles * p.kvHeads, sms = deviceSMs();
+  long long longest = p.reach;
+  if (p.window + p.sinks + kCtaRows < longest) longest = p.window + p.sinks + kCtaRows;
+  long long splits = ctas >= sms ? 1 : sms / ctas;
+  const long long most2 = (longest + 2 * kKeys - 1) / (2 * kKeys);
+  if (splits > most2) splits = most2;
+  if (splits > kMaxSplits) splits = kMaxSplits;
+  l.splits = splits < 1 ? 1 : (int)splits;
+  return l;
+}
+template <int D> long long bytesOf(const PagedArgs& p, const Launch& l) {
+  const long long pairs = l.tiles * p.kvHeads;
+  return l.splits == 1 ? 0 : pairs * 16 + pairs * 2 * l.splits * Config<D>::kPart * 4;
+}
+
+template <typename T, int D>
+int launch(const PagedArgs& p, int doneRows, void* workspace, long long bytes, cudaStream_t st) {
+  using C = Config<D>;
+  CUtensorMap mk, mv;
+  ChunkArgs a{};
+  a.p = p;
+  a.doneRows = doneRows;
+  a.boxRows = p.pageSize < kKeys ? (int)p.pageSize : kKeys;
+  while ((1LL << a.pageShift) < p.pageSize) ++a.pageShift;
+  if (!makePageMap(&mk, p.k, p.dtype, p, p.kcSp, p.kcSn, p.kcSh, a.boxRows) || !makePageMap(&mv, p.v, p.dtype, p, p.vcSp, p.vcSn, p.vcSh, a.boxRows))
+    return setError(LLC_ERR_CUDA, "llc cuda: cuTensorMapEncodeTiled rejected the cache");
+  // a scale of 0 becomes one that no score survives: 0 times a masked score's -inf would be NaN
+  a.scaleAbs = fabsf(p.scaleLog2) > 1e-37f || p.scaleLog2 != p.scaleLog2 ? fabsf(p.scaleLog2) : 1e-37f;
+  a.signQ = p.scaleLog2 < 0.f ? -1.f : 1.f;
+  Launch l = launchOf(p);
+  if (!workspace || bytes < bytesOf<D>(p, l)) l.splits = 1;
+  a.splits = l.splits;
+  const long long pairs = l.tiles * p.kvHeads;
+  a.records = static_cast<int4*>(workspace);
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + pairs * 16);
+  if (l.tiles > 65535 || (long long)p.kvHeads * l.splits > 0x7FFFFFFFLL) return setError(LLC_ERR_UNSUPPORTED, "llc argument: paged_attention too many tiles");
+  static DeviceOnce configured;
+  const int dev = currentDevice();
+  if (!configured.test(dev)) {
+    LLC_CUDA_CHECK(cudaFuncSetAttribute(paged_chunk_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    configured.set(dev);
+  }
+  paged_chunk_kernel<T, D><<<dim3((unsigned)(p.kvHeads * l.splits), (unsigned)l.tiles), kThreads, C::kSmem, st>>>(mk, mv, a);
+  LLC_LAUNCH_CHECK("paged_chunk_kernel");
+  if (l.splits > 1) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(2 * pairs));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    LLC_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_chunk_join_kernel<T, D>, a));
+  }
+  return LLC_OK;
+}
+
+}  // namespace
+
+// The sequences of more than doneRows rows (new tokens x query heads of a key head).
+long long pagedChunkWorkspace(const PagedArgs& p) { return p.d == 64 ? bytesOf<64>(p, launchOf(p)) : bytesOf<128>(p, launchOf(p)); }
+int pagedChunk(const PagedArgs& p, int doneRows, void* workspace, long long bytes, cudaStream_t st) {
+  if (p.dtype == LLC_BFLOAT16)
+    return p.d == 64 ? launch<__nv_bfloat16, 64>(p, doneRows, workspace, bytes, st) : launch<__nv_bfloat16, 128>(p, doneRows, workspace, bytes, st);
+  return p.d == 64 ? launch<__half, 64>(p, doneRows, workspace, bytes, st) : launch<__half, 128>(p, doneRows, workspace, bytes, st);
+}
+
+int pagedChunkStatus() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_pagedChunkStatus, sizeof(int)) != cudaSuccess) return -1;
+  if (v) cudaMemcpyToSymbol(g_pagedChunkStatus, &zero, sizeof(int));
+  return v;
+}
+
+}  // namespace llc

@@ -11,8 +11,6 @@
 // Work: the blocks of 64 keys of all (sequence, key head) pairs form one line, cut into equal shares, one a CTA, so that
 // ragged batches and single long sequences load every SM alike.  A pair that is cut leaves partial sums in the workspace,
 // which a second kernel joins (launched early, it waits for this one on the device).
-#include <type_traits>
-
 #include "paged_attention.cuh"
 #include "tc_common.cuh"
 #include "tensor_map.h"
@@ -26,7 +24,6 @@ using namespace tc;
 constexpr int kConsumers = 4;                      // warps
 constexpr int kThreads = (kConsumers + 1) * 32;
 constexpr int kKeys = 64;                          // keys of a block (and of a stage)
-constexpr float kRescaleStep = 8.f;                // the running maximum follows in steps larger than 2^8 only
 
 template <int D, int MT> struct Config {
   static constexpr int kRows = 16 * MT;
@@ -51,22 +48,17 @@ struct DecodeArgs {
   float* slots;                // [2 * CTAs][kSlot]
 };
 
-// The blocks of keys that a sequence's tokens see: sinkBlocks from the start, then [firstBlock, endBlock).
-struct Blocks { int sinkBlocks, firstBlock, count; long long lo, sinkEnd, hi; };   // visible to some token: [0, sinkEnd) and [lo, hi)
-__device__ __forceinline__ Blocks blocksOf(const PagedArgs& p, const Sequence& s, int maxRows) {
-  Blocks b{};
-  if (s.n == 0 || s.n * p.group > maxRows) return b;
-  const long long p0 = s.len - s.n;                // place of the first token
-  b.hi = s.len;
-  b.lo = p0 + 1 - p.window > 0 ? p0 + 1 - p.window : 0;
-  if (b.lo > b.hi) b.lo = b.hi;
-  b.sinkEnd = p.sinks < b.lo ? p.sinks : b.lo;
-  b.firstBlock = (int)(b.lo / kKeys);
-  b.sinkBlocks = (int)((b.sinkEnd + kKeys - 1) / kKeys);
-  if (b.sinkBlocks > b.firstBlock) b.sinkBlocks = b.firstBlock;
-  b.count = b.sinkBlocks + (int)((b.hi + kKeys - 1) / kKeys) - b.firstBlock;
-  if (b.count < 1) b.count = 1;                    // nothing is visible: one empty block writes the zeros
+// The blocks of keys of one key head of a sequence; one empty block where nothing is visible, which writes the zeros; none where the
+// sequence has no rows, or more than this kernel takes.
+__device__ __forceinline__ Blocks blocksOf(const PagedArgs& p, const Sequence& s, const Seen& seen, int maxRows) {
+  if (s.n == 0 || s.n * p.group > maxRows) return Blocks{0, 0, 0};
+  Blocks b = blocksOf(seen, kKeys);
+  if (b.count < 1) b.count = 1;
   return b;
+}
+__device__ __forceinline__ int countOf(const PagedArgs& p, int b, int maxRows) {
+  const Sequence s = sequenceOf(p, b);
+  return blocksOf(p, s, seenBy(p, s.len - s.n, s.len - 1), maxRows).count;
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t* r) {
@@ -84,19 +76,6 @@ template <> __device__ __forceinline__ void mma16816<__half>(float* c, const uin
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) { __nv_bfloat162 v = __floats2bfloat162_rn(x, y); return *reinterpret_cast<uint32_t*>(&v); }
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) { __half2 v = __floats2half2_rn(x, y); return *reinterpret_cast<uint32_t*>(&v); }
-// Weights are rounded to the tensors' type for the second product.  f16 weights are kept 2^7 times larger, so that a weight loses
-// bits to f16's subnormals only below 2^-21 of the largest (2^7 x 2^8 of lag stays below 65504).
-template <typename T> constexpr float weightShift() { return std::is_same<T, __half>::value ? 7.f : 0.f; }
-
-// Whether one of two packed numbers is NaN or infinite.
-template <typename T> __device__ __forceinline__ bool notFinite(uint32_t x) {
-  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  return (x & e) == e || (x & (e << 16)) == (e << 16);
-}
-
 __device__ __forceinline__ void consumerBarrier() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory"); }
 
 template <typename T, int D, int MT>
@@ -137,13 +116,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
     b = blockIdx.x / p.kvHeads;
     h = blockIdx.x - b * p.kvHeads;
     unit = 0;
-    left = blocksOf(p, sequenceOf(p, b), C::kRows).count;
+    left = countOf(p, b, C::kRows);
   } else {
     const int per = (p.batch + kConsumers * 32 - 1) / (kConsumers * 32);
     const int first = threadIdx.x * per;
     long long mine = 0, before = 0;
     if (warp < kConsumers) {
-      for (int i = first; i < first + per && i < p.batch; ++i) mine += blocksOf(p, sequenceOf(p, i), C::kRows).count;
+      for (int i = first; i < first + per && i < p.batch; ++i) mine += countOf(p, i, C::kRows);
       long long run = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += x; }
@@ -161,7 +140,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
     const long long start = blockIdx.x * share;
     if (warp < kConsumers && start >= before * p.kvHeads && start < (before + mine) * p.kvHeads) {
       for (int i = first; i < first + per && i < p.batch; ++i) {
-        const long long c = blocksOf(p, sequenceOf(p, i), C::kRows).count;
+        const long long c = countOf(p, i, C::kRows);
         if (start < (before + c) * p.kvHeads) { *sSeq = i; sStart[0] = start - before * p.kvHeads; break; }
         before += c;
       }
@@ -173,7 +152,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
       if (threadIdx.x == 0) a.records[blockIdx.x] = make_int4(-1, 0, 0, 0);
       return;
     }
-    const int c = blocksOf(p, sequenceOf(p, b), C::kRows).count;
+    const int c = countOf(p, b, C::kRows);
     h = (int)(sStart[0] / c);
     unit = sStart[0] - (long long)h * c;
   }
@@ -187,17 +166,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
     const int box = lane % boxes, half = lane / boxes % (D / 64), which = lane / (boxes * (D / 64));   // this lane's load of every stage
     while (left > 0 && ok) {
       const Sequence s = sequenceOf(p, b);
-      const Blocks bl = blocksOf(p, s, C::kRows);
+      const Seen seen = seenBy(p, s.len - s.n, s.len - 1);
+      const Blocks bl = blocksOf(p, s, seen, C::kRows);
       if (bl.count == 0) { ++b; h = 0; continue; }
       const long long end = unit + left < bl.count ? unit + left : bl.count;
       left -= end - unit;
       for (; unit < end && ok; ++unit, ++it) {
         const int st = it % C::kStages;
-        const long long j = (unit < bl.sinkBlocks ? unit : unit - bl.sinkBlocks + bl.firstBlock) * kKeys + (long long)box * a.boxRows;
+        const long long j = keyOf(bl, unit, kKeys) + (long long)box * a.boxRows;
         // a box that no token sees any key of is not looked up: it reads as zeros, as does one with a bad page number
-        const bool seen = lane < loads && (j < bl.sinkEnd || (j < bl.hi && j + a.boxRows > bl.lo));
+        const bool wanted = lane < loads && (j < seen.sinkEnd || (j < seen.hi && j + a.boxRows > seen.lo));
         long long page = -1;
-        if (seen) {
+        if (wanted) {
           page = pageOf(p, b, j >> a.pageShift);
           if (page < 0 && which == 0 && half == 0 && p.badPages) atomicAdd(p.badPages, 1);
         }
@@ -231,7 +211,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
   int4 record = make_int4(-1, 0, 0, 0);
   while (left > 0) {
     const Sequence s = sequenceOf(p, b);
-    const Blocks bl = blocksOf(p, s, C::kRows);
+    const Seen seen = seenBy(p, s.len - s.n, s.len - 1);
+    const Blocks bl = blocksOf(p, s, seen, C::kRows);
     if (bl.count == 0) { ++b; h = 0; continue; }
     const long long begin = unit, end = unit + left < bl.count ? unit + left : bl.count;
     left -= end - unit;
@@ -263,7 +244,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
     }
     for (; unit < end; ++unit, ++it) {
       const int st = it % C::kStages;
-      const long long j0 = (unit < bl.sinkBlocks ? unit : unit - bl.sinkBlocks + bl.firstBlock) * kKeys + warp * 16;   // this warp's keys
+      const long long j0 = keyOf(bl, unit, kKeys) + warp * 16;   // this warp's keys
       if (ok && !mbarWait(&full[st], (it / C::kStages) & 1u, abortWord)) { ok = false; atomicExch(&g_pagedDecodeStatus, 9); }
       __syncwarp();
       const uint32_t kAddr = kBase + st * C::kStage, vAddr = vBase + st * C::kStage;
@@ -294,7 +275,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
               if (!sees) hidden |= 1u << (mt * 8 + r * 4 + i);
             }
           // a value that nobody sees may be NaN, and 0 x NaN is NaN: it is taken as 0
-          if (!(j < bl.hi && (j >= bl.lo || j < bl.sinkEnd))) vMask[i >> 1] &= (i & 1) ? 0x0000ffffu : 0xffff0000u;
+          if (!(j < seen.hi && (j >= seen.lo || j < seen.sinkEnd))) vMask[i >> 1] &= (i & 1) ? 0x0000ffffu : 0xffff0000u;
         }
       }
       uint32_t pf[MT][4];

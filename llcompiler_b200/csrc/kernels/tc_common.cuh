@@ -220,6 +220,13 @@ __device__ __forceinline__ void mmaSS(uint32_t tmemD, uint64_t descA, uint64_t d
         ::"r"(tmemD), "l"(descA), "l"(descB), "r"(idesc), "r"(accumulate) : "memory");
   }
 }
+// The A operand from tensor memory (16-bit types: two neighbours along K in a 32-bit column, 16 of them a step in 8 columns).
+__device__ __forceinline__ void mmaTS(uint32_t tmemD, uint32_t tmemA, uint64_t descB, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmemD), "r"(tmemA), "l"(descB), "r"(idesc), "r"(accumulate) : "memory");
+}
 // One MMA over a CTA pair: M = 256, CTA r holds rows 128 r..+127 of A and of the accumulator and half r of the rows of B;
 // issued by CTA 0 with descriptors that name the same places in both CTAs.
 template <bool TF32>
@@ -284,6 +291,21 @@ __device__ __forceinline__ void tmemWait32(uint32_t* r) {
                  "+r"(r[30]), "+r"(r[31])
                :: "memory");
 }
+
+// 32 lanes x 32 consecutive columns into tensor memory: thread i of the warp writes row (lane base + i).  Complete for the
+// thread after tmemStoreWait.
+__device__ __forceinline__ void tmemStore32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+        "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 32 lanes x N consecutive fp32 columns (N = 16 or 32).
 template <int N> __device__ __forceinline__ void tmemLoadCols(uint32_t taddr, float* v);
