@@ -115,10 +115,10 @@ int checkAndFill(const LlcPagedAttentionParams* p, PagedArgs* a) {
   a->qSt = p->q_st; a->qSh = p->q_sh; a->oSt = p->o_st; a->oSh = p->o_sh;
   a->kcSp = p->kc_sp; a->kcSn = p->kc_sn; a->kcSh = p->kc_sh; a->vcSp = p->vc_sp; a->vcSn = p->vc_sn; a->vcSh = p->vc_sh;
   a->tableS0 = p->table_s0; a->tokens = p->tokens; a->numPages = p->num_pages; a->pageSize = p->page_size;
-  a->reach = p->table_width * p->page_size;
+  a->reach = (int)(p->table_width * p->page_size);
   a->maxQ = p->max_q < p->tokens ? p->max_q : p->tokens;
-  a->window = p->window > 0 && p->window < a->reach ? p->window : a->reach + 1;
-  a->sinks = p->sinks < a->reach ? p->sinks : a->reach;
+  a->window = p->window > 0 && p->window < a->reach ? (int)p->window : a->reach + 1;
+  a->sinks = p->sinks < a->reach ? (int)p->sinks : a->reach;
   a->batch = (int)p->batch; a->heads = (int)p->heads; a->kvHeads = (int)p->kv_heads; a->group = (int)(p->heads / p->kv_heads);
   a->d = (int)p->d; a->dtype = p->dtype;
   a->scaleLog2 = p->scale * 1.4426950408889634f;
@@ -136,10 +136,11 @@ bool tensorTypes(const PagedArgs& a) {
 }
 
 // Rows of a sequence up to which the decode kernel takes it.  A call whose sequences all have at most 32 rows runs there alone; beside
-// longer chunks it takes the sequences of single tokens (16 rows, which leave two CTAs on an SM, or 32 for large groups).
+// longer chunks of other sequences it takes the sequences of single tokens (16 rows, which leave two CTAs on an SM, or 32 for large groups).
 int decodeRows(const PagedArgs& a) {
   const long long rows = a.maxQ * a.group;
   if (rows <= 32) return rows <= 16 ? 16 : 32;
+  if (a.batch == 1) return 0;
   return a.group <= 16 ? 16 : a.group <= 32 ? 32 : 0;
 }
 

@@ -13,21 +13,21 @@ struct PagedArgs {
   const void* q; const void* k; const void* v; void* out;
   const int* table; const int* qStart; const int* kvLen; int* badPages;
   long long qSt, qSh, oSt, oSh, kcSp, kcSn, kcSh, vcSp, vcSn, vcSh, tableS0;
-  long long tokens, numPages, pageSize, reach, maxQ;
-  long long window, sinks;             // window: past the longest sequence where the caller has none
+  long long tokens, numPages, pageSize, maxQ;
+  int reach, window, sinks;            // slots that a row of the page table names, below 2^31 - 256; window: reach + 1 where the caller has none
   int batch, heads, kvHeads, group, d, dtype;
   float scaleLog2;                     // scale * log2(e): the softmax is taken to base 2
 };
 
 // One sequence: rows begin .. begin + n - 1 of q, the i-th of them at place len - n + i.
-struct Sequence { long long begin, n, len; };
+struct Sequence { long long begin; int n, len; };
 __device__ __forceinline__ Sequence sequenceOf(const PagedArgs& p, int b) {
   Sequence s;
   const long long lo = p.qStart[b], hi = p.qStart[b + 1];
   s.begin = lo < 0 ? 0 : lo;
-  s.n = (hi > p.tokens ? p.tokens : hi) - s.begin;
-  if (s.n < 0 || s.n > p.maxQ) s.n = 0;
-  const long long len = p.kvLen[b];
+  const long long n = (hi > p.tokens ? p.tokens : hi) - s.begin;
+  s.n = n < 0 || n > p.maxQ ? 0 : (int)n;
+  const int len = p.kvLen[b];
   s.len = len < 0 ? 0 : len > p.reach ? p.reach : len;
   return s;
 }
@@ -38,11 +38,13 @@ __device__ __forceinline__ long long pageOf(const PagedArgs& p, int b, long long
   return page >= 0 && page < p.numPages ? page : -1;
 }
 
-// The keys that tokens at places first .. last of a sequence of len keys see, some of them at least: [0, sinkEnd) and [lo, hi).
-struct Seen { long long sinkEnd, lo, hi; };
-__device__ __forceinline__ Seen seenBy(const PagedArgs& p, long long first, long long last) {
+// The keys that tokens at places first .. last of a sequence see, some of them at least: [0, sinkEnd) and [lo, hi).  Places below 0
+// (more new tokens than the length says) see nothing; they are clipped to -1, so that all of this fits 32 bits.
+struct Seen { int sinkEnd, lo, hi; };
+__device__ __forceinline__ int clipPlace(long long place) { return place < 0 ? -1 : (int)place; }
+__device__ __forceinline__ Seen seenBy(const PagedArgs& p, int first, int last) {
   Seen s;
-  s.hi = last + 1 > 0 ? last + 1 : 0;
+  s.hi = last + 1;
   s.lo = first + 1 - p.window > 0 ? first + 1 - p.window : 0;
   if (s.lo > s.hi) s.lo = s.hi;
   s.sinkEnd = p.sinks < s.lo ? p.sinks : s.lo;
@@ -52,13 +54,13 @@ __device__ __forceinline__ Seen seenBy(const PagedArgs& p, long long first, long
 struct Blocks { int sink, first, count; };
 __device__ __forceinline__ Blocks blocksOf(const Seen& s, int keys) {
   Blocks b;
-  b.first = (int)(s.lo / keys);
-  b.sink = (int)((s.sinkEnd + keys - 1) / keys);
+  b.first = s.lo / keys;
+  b.sink = (s.sinkEnd + keys - 1) / keys;
   if (b.sink > b.first) b.sink = b.first;
-  b.count = b.sink + (int)((s.hi + keys - 1) / keys) - b.first;
+  b.count = b.sink + (s.hi + keys - 1) / keys - b.first;
   return b;
 }
-__device__ __forceinline__ long long keyOf(const Blocks& b, long long unit, int keys) { return (unit < b.sink ? unit : unit - b.sink + b.first) * keys; }
+__device__ __forceinline__ int keyOf(const Blocks& b, int unit, int keys) { return (unit < b.sink ? unit : unit - b.sink + b.first) * keys; }
 
 // Two numbers rounded to T, and whether one of two packed numbers is NaN or infinite.
 template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);

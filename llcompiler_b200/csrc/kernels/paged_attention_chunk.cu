@@ -3,9 +3,10 @@
 // (token, query head) pairs of one key head, token-major, so that all query heads of a group read the keys once and a tile's rows
 // differ little in what they see.
 // A CTA takes two tiles of 128 rows and walks the blocks of 128 keys that either sees:
-//   8 softmax warps   four a tile, one thread a row: the row's 128 scores come out of tensor memory into registers once; maximum,
+//   16 softmax warps  eight a tile, two threads a row: a thread's 64 scores come out of tensor memory into registers once; maximum,
 //                     2^x, sum, weights back into tensor memory as 16-bit numbers over the scores' own columns, from where the
-//                     second product takes them as its A operand (they never cross shared memory)
+//                     second product takes them as its A operand (they never cross shared memory).  (One thread a row, eight
+//                     warps: the schedulers found a warp to issue from in 31 % of the cycles.)
 //   loader warp       one lane a page box: TMA loads of K and V blocks into a ring of slots
 //   issuer warp       S_A, S_B, then for every block: O_A += P_A V, S_A of the next block, O_B += P_B V, S_B of the next block, so that
 //                     one tile's softmax runs under the other tile's products
@@ -22,7 +23,8 @@ __device__ int g_pagedChunkStatus = 0;    // non-zero after a bounded wait gave 
 namespace {
 using namespace tc;
 
-constexpr int kThreads = 384;             // 8 softmax warps, loader, issuer, two idle warps that fill the warpgroup
+constexpr int kSoftmaxWarps = 16, kLoaderWarp = 16, kIssuerWarp = 17;
+constexpr int kThreads = 20 * 32;          // the last two warps are idle: they fill the warpgroup that gives registers away
 constexpr int kTileRows = 128, kCtaRows = 256, kKeys = 128;
 constexpr int kMaxSplits = 32;
 
@@ -30,10 +32,10 @@ template <int D> struct Config {
   static constexpr int kAtom = 128 * 128;             // bytes of 128 rows x 64 elements
   static constexpr int kTile = kAtom * (D / 64);      // Q of a tile, K or V of a block
   static constexpr int kSlots = D == 128 ? 5 : 10;
-  static constexpr int kMisc = 1024;
+  static constexpr int kMisc = 3072;                  // barriers, then the row statistics that a row's two threads exchange
   static constexpr int kSmem = 2 * kTile + kSlots * kTile + kMisc;
   static constexpr int kPart = kTileRows * (D + 2);   // floats of a tile's partial sums: O as [D / 4][128 rows] vectors, then m, then l
-  static_assert(kSmem + 1024 <= 228 * 1024, "one CTA an SM");
+  static_assert(kSmem <= 227 * 1024, "one CTA an SM");
 };
 // Columns of tensor memory.
 constexpr uint32_t kColS = 0, kColO = 256;
@@ -47,39 +49,102 @@ struct ChunkArgs {
   float* parts;                // [tiles * key heads][2][splits][kPart]
 };
 
-// What a tile's rows see, and which blocks it takes part in.
+// What a tile's rows see.
 struct Tile {
-  long long first, last;       // places of its first and last token
+  int first, last;             // places of its first and last token
   Seen seen;
-  __device__ bool active(long long j0) const { return j0 < seen.sinkEnd || (j0 < seen.hi && j0 + kKeys > seen.lo); }
 };
 __device__ __forceinline__ Tile tileOf(const PagedArgs& p, const Sequence& s, long long row0, long long rows) {
   Tile t;
   const long long rowEnd = row0 + kTileRows < rows ? row0 + kTileRows : rows;
   if (row0 >= rowEnd) { t.first = 0; t.last = -1; t.seen = Seen{0, 0, 0}; return t; }
-  t.first = s.len - s.n + row0 / p.group;
-  t.last = s.len - s.n + (rowEnd - 1) / p.group;
+  t.first = clipPlace((long long)s.len - s.n + row0 / p.group);
+  t.last = clipPlace((long long)s.len - s.n + (rowEnd - 1) / p.group);
   t.seen = seenBy(p, t.first, t.last);
   return t;
 }
+// The same in units (positions in the CTA's list of blocks): a tile takes part in units u < sink and lo <= u < hi, and every row of it sees
+// all keys of the units u < wholeSink and wholeLo <= u < wholeHi.
+struct Units { int sink, lo, hi, wholeSink, wholeLo, wholeHi; };
+__device__ __forceinline__ Units unitsOf(const PagedArgs& p, const Tile& t, const Blocks& bl) {
+  Units n;
+  const int shift = bl.sink - bl.first;               // unit of a block of the second part; 0 where the two parts meet
+  n.sink = (t.seen.sinkEnd + kKeys - 1) / kKeys;
+  n.lo = t.seen.lo / kKeys + shift;
+  if (n.lo < n.sink) n.lo = n.sink;
+  n.hi = (t.seen.hi + kKeys - 1) / kKeys + shift;
+  if (t.seen.hi == 0) n.sink = n.lo = n.hi = 0;
+  const int before = t.first + 1;                     // keys that lie before every row's own place or on it
+  n.wholeSink = (p.sinks < before ? p.sinks : before) / kKeys;
+  n.wholeHi = before / kKeys + shift;
+  n.wholeLo = (t.last - p.window >= 0 ? (t.last - p.window) / kKeys + 1 : 0) + shift;
+  return n;
+}
+
+// What a CTA does, worked out by one thread and read from shared memory where it is needed: kept in registers it would displace scores.
+struct Plan {
+  Units units[2];              // of the two tiles
+  Blocks bl;
+  Seen seen;                   // by the rows of both
+  int begin, end;              // units of this CTA's part of the keys
+  int seq, tile;               // sequence (-1: nothing to do) and pair of tiles
+  int n, len;                  // of the sequence
+  long long row0, rows, qBegin;
+};
+
+// Barriers by their shared-memory address (a generic pointer costs two registers and a conversion at every use).
+__device__ __forceinline__ bool waitAt(uint32_t bar, uint32_t parity, uint32_t abortAt) {
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+    if ((i & 255) == 255) {
+      uint32_t gone;
+      asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(gone) : "r"(abortAt) : "memory");
+      if (gone) return false;
+    }
+  }
+  asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abortAt), "r"(1) : "memory");
+  return false;
+}
+__device__ __forceinline__ void arriveAt(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void commitAt(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 __device__ __forceinline__ long long tilesOf(const PagedArgs& p, int b, int doneRows) {
-  const long long rows = sequenceOf(p, b).n * p.group;
+  const long long rows = (long long)sequenceOf(p, b).n * p.group;
   return rows <= doneRows ? 0 : (rows + kCtaRows - 1) / kCtaRows;
 }
+
+// Barriers of the two warps that share 32 rows; the first also tells whether any of the 64 threads said yes.
+__device__ __forceinline__ void pairBarrier(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool barrierOr(int id, bool yes) {
+  int any;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 64, p;\n\tselp.s32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"(id), "r"((int)yes) : "memory");
+  return any != 0;
+}
+__device__ __forceinline__ void storeShared(uint32_t at, float x) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(x) : "memory"); }
+__device__ __forceinline__ float loadShared(uint32_t at) { float x; asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory"); return x; }
+__device__ __forceinline__ uint32_t bitsBelow(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 // A row's sum over its visible keys among the blocks [begin, end) by multiply-adds, one warp a row: lane l gets elements l, l + 32, ...
 // Taken for a row whose sum came out NaN or infinite though its weights are finite: some value in the blocks is, and the products
 // multiply every value of a block by every row's weights, those that are 0 because the row does not see the value too.
 template <typename T, int D>
-__device__ __noinline__ void sumRow(const ChunkArgs& a, int b, int h, long long qOff, long long pos, Blocks bl, int begin, int end, float base, float* o) {
+__device__ __noinline__ void sumRow(const ChunkArgs& a, int b, int h, long long qOff, int pos, Blocks bl, int begin, int end, float base, float* o) {
   const PagedArgs& p = a.p;
   const int lane = threadIdx.x & 31;
   float q[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) { q[i] = (float)reinterpret_cast<const T*>(p.q)[qOff + lane + 32 * i] * a.signQ; o[i] = 0.f; }
   for (int u = begin; u < end; ++u) {
-    const long long j0 = keyOf(bl, u, kKeys);
-    for (long long j = j0; j < j0 + kKeys; ++j) {
+    const int j0 = keyOf(bl, u, kKeys);
+    for (int j = j0; j < j0 + kKeys; ++j) {
       if (!(j <= pos && (pos - j < p.window || j < p.sinks))) continue;
       const long long page = pageOf(p, b, j >> a.pageShift), slot = j & ((1 << a.pageShift) - 1);
       if (page < 0) continue;                         // its values are zeros
@@ -111,11 +176,18 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
   uint64_t* qReady = oFull + 2;                       // both tiles of Q written
   uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(misc + 256);
   volatile int* abortWord = reinterpret_cast<volatile int*>(misc + 260);
-  int* sSeq = reinterpret_cast<int*>(misc + 264);
-  int* sTile = sSeq + 1;
-  long long* sScan = reinterpret_cast<long long*>(misc + 272);   // [12]
+  long long* sScan = reinterpret_cast<long long*>(misc + 264);   // [20]
+  Plan* plan = reinterpret_cast<Plan*>(misc + 512);
+  float* sRow = reinterpret_cast<float*>(misc + 1024);           // [2 tiles][2 halves][128]
   const PagedArgs& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (smemAddr(smem) & 1023) {                        // the swizzled tiles need it; no static shared memory lies before them
+    if (threadIdx.x == 0) {
+      atomicExch(&g_pagedChunkStatus, 10);
+      if (a.splits > 1 && blockIdx.x % a.splits == 0) a.records[(long long)blockIdx.y * p.kvHeads + blockIdx.x / a.splits] = make_int4(-1, 0, 0, 0);
+    }
+    return;
+  }
 
   // Which sequence and tiles: blockIdx.x = head and part of the keys, blockIdx.y = tile pair, counted from the last, which sees the
   // most keys of its sequence.
@@ -129,10 +201,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += x; }
     if (lane == 31) sScan[warp] = run;
     if (threadIdx.x == 0) {
-      *sSeq = -1;
+      plan->seq = -1;
       for (int i = 0; i < C::kSlots; ++i) { mbarInit(&kvFull[i], 1); mbarInit(&kvEmpty[i], 1); }
-      for (int t = 0; t < 2; ++t) { mbarInit(&sFull[t], 1); mbarInit(&pReady[t], 4); mbarInit(&oFull[t], 1); }
-      mbarInit(qReady, 8);
+      for (int t = 0; t < 2; ++t) { mbarInit(&sFull[t], 1); mbarInit(&pReady[t], kSoftmaxWarps / 2); mbarInit(&oFull[t], 1); }
+      mbarInit(qReady, kSoftmaxWarps);
       *abortWord = 0;
       fenceBarrierInit();
     }
@@ -141,46 +213,52 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     for (int w = 0; w < kThreads / 32; ++w) { if (w < warp) before += sScan[w]; all += sScan[w]; }
     const long long want = all - 1 - (long long)blockIdx.y;
     if (want >= before && want < before + mine) {
-      for (int i = first; i < first + per && i < p.batch; ++i) {
+      int i = first;
+      for (; i < first + per; ++i) {
         const long long c = tilesOf(p, i, a.doneRows);
-        if (want < before + c) { *sSeq = i; *sTile = (int)(want - before); break; }
+        if (want < before + c) break;
         before += c;
       }
+      const Sequence s = sequenceOf(p, i);
+      const long long rows = (long long)s.n * p.group, row0 = (want - before) * kCtaRows;
+      const Tile tile0 = tileOf(p, s, row0, rows), tile1 = tileOf(p, s, row0 + kTileRows, rows);
+      plan->seen = seenBy(p, tile0.first, tile1.last >= 0 ? tile1.last : tile0.last);
+      const Blocks bl = blocksOf(plan->seen, kKeys);
+      const int share = (bl.count + a.splits - 1) / a.splits, begin = share * split < bl.count ? share * split : bl.count;
+      plan->units[0] = unitsOf(p, tile0, bl);
+      plan->units[1] = unitsOf(p, tile1, bl);
+      plan->bl = bl;
+      plan->begin = begin;
+      plan->end = begin + share < bl.count ? begin + share : bl.count;
+      plan->seq = i; plan->tile = (int)(want - before); plan->n = s.n; plan->len = s.len;
+      plan->row0 = row0; plan->rows = rows; plan->qBegin = s.begin;
     }
     __syncthreads();
   }
-  const int b = *sSeq;
   const long long pair = (long long)blockIdx.y * p.kvHeads + h;
-  if (a.splits > 1 && split == 0 && threadIdx.x == 0) a.records[pair] = make_int4(b, b < 0 ? 0 : *sTile, 0, 0);
-  if (b < 0) return;                                  // fewer tiles than the grid has room for
-  if (smemAddr(smem) & 1023) {                        // the swizzled tiles need it; no static shared memory lies before them
-    if (threadIdx.x == 0) { atomicExch(&g_pagedChunkStatus, 10); if (a.splits > 1 && split == 0) a.records[pair] = make_int4(-1, 0, 0, 0); }
-    return;
-  }
-  const Sequence s = sequenceOf(p, b);
-  const long long rows = s.n * p.group, row0 = (long long)*sTile * kCtaRows;
-  const Tile tile0 = tileOf(p, s, row0, rows), tile1 = tileOf(p, s, row0 + kTileRows, rows);
-  const Seen seen = seenBy(p, tile0.first, tile1.last >= 0 ? tile1.last : tile0.last);
-  const Blocks bl = blocksOf(seen, kKeys);
-  const int share = (bl.count + a.splits - 1) / a.splits;
-  const int begin = share * split < bl.count ? share * split : bl.count, end = begin + share < bl.count ? begin + share : bl.count;
+  if (a.splits > 1 && split == 0 && threadIdx.x == 0) a.records[pair] = make_int4(plan->seq, plan->tile, 0, 0);
+  if (plan->seq < 0) return;                          // fewer tiles than the grid has room for
 
-  if (warp == 9) tmemAlloc(tmemSlot, 512);
+  if (warp == kIssuerWarp) tmemAlloc(tmemSlot, 512);
   tcFenceBefore();
   __syncthreads();
   tcFenceAfter();
   const uint32_t tmem = *tmemSlot;
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 8) {
+  // Registers: 96 a thread at launch, 640 threads; 104 for the 512 softmax threads and 64 for the other 128 make the same sum.
+  if (warp >= kSoftmaxWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == kLoaderWarp) {
       // ---------------------------------------------------------------- loader: items K, V, K, V, ...
       if (lane == 0) { prefetchTensorMap(&mapK); prefetchTensorMap(&mapV); }
       const int boxes = kKeys / a.boxRows, loads = boxes * (D / 64), box = lane % boxes, half = lane / boxes;
       bool ok = true;
       uint32_t item = 0;
+      const int b = plan->seq, begin = plan->begin, end = plan->end;
+      const Blocks bl = plan->bl;
+      const Seen seen = plan->seen;
       auto lookUp = [&](int u) -> long long {
-        const long long j = keyOf(bl, u, kKeys) + (long long)box * a.boxRows;
+        const int j = keyOf(bl, u, kKeys) + box * a.boxRows;
         // a box that no row sees any key of is not looked up: it reads as zeros, as does one with a bad page number
         if (lane >= loads || !(j < seen.sinkEnd || (j < seen.hi && j + a.boxRows > seen.lo))) return -1;
         const long long page = pageOf(p, b, j >> a.pageShift);
@@ -207,54 +285,75 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
         if (lane == 0) atomicExch(&g_pagedChunkStatus, 10);
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);   // copies in flight land before the CTA gives its memory back
       }
-    } else if (warp == 9 && lane == 0) {
+    } else if (warp == kIssuerWarp && lane == 0) {
       // ---------------------------------------------------------------- issuer
+      // One thread feeds the tensor pipe: descriptors are built once, a slot only adds its offset, and the loop has no division.
       constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
       constexpr uint32_t idescS = instrDesc(fmt, kTileRows, kKeys, 0, 0), idescO = instrDesc(fmt, kTileRows, D, 0, 1);
-      bool ok = mbarWait(qReady, 0, abortWord);
-      uint32_t weights[2] = {0, 0};                   // blocks whose weights a tile's warps have handed over
-      bool started[2] = {false, false};
-      auto active = [&](int t, int u) { return (t ? tile1 : tile0).active(keyOf(bl, u, kKeys)); };
-      auto slotWait = [&](uint32_t item) { ok = ok && mbarWait(&kvFull[item % C::kSlots], (item / C::kSlots) & 1u, abortWord); };
-      auto issueS = [&](int t, uint32_t item) {
-        const uint32_t q = smemAddr(sQ + t * C::kTile), k = smemAddr(ring + (item % C::kSlots) * C::kTile);
+      const Units n0 = plan->units[0], n1 = plan->units[1];
+      const int begin = plan->begin, end = plan->end;
+      const uint64_t descQ = smemDescKMajorSw128(smemAddr(sQ)), descK = smemDescKMajorSw128(smemAddr(ring)), descV = smemDescMnMajorSw128(smemAddr(ring), C::kAtom);
+      const uint32_t full = smemAddr(kvFull), empty = smemAddr(kvEmpty), sf = smemAddr(sFull), pr = smemAddr(pReady), gone = smemAddr((const void*)abortWord);
+      constexpr uint32_t kAtom16 = C::kAtom >> 4, kTile16 = C::kTile >> 4;
+      bool ok = waitAt(smemAddr(qReady), 0, gone);
+      auto active = [&](const Units& n, int u) { return u < n.sink || (u >= n.lo && u < n.hi); };
+      auto issueS = [&](int t, uint32_t slot) {
+        const uint64_t q = descQ + t * kTile16, k = descK + slot * kTile16;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
-          mmaSS<false>(tmem + kColS + t * kKeys, smemDescKMajorSw128(q + (ks / 4) * C::kAtom) + 2 * (ks % 4), smemDescKMajorSw128(k + (ks / 4) * C::kAtom) + 2 * (ks % 4), idescS,
-                       ks > 0 ? 1u : 0u);
-        mmaCommit(&sFull[t]);
+          mmaSS<false>(tmem + kColS + t * kKeys, q + (ks / 4) * kAtom16 + 2 * (ks % 4), k + (ks / 4) * kAtom16 + 2 * (ks % 4), idescS, ks > 0 ? 1u : 0u);
+        commitAt(sf + 8 * t);
       };
+      auto issueO = [&](int t, uint32_t slot, bool more) {
+        const uint64_t v = descV + slot * kTile16;
+#pragma unroll
+        for (int ks = 0; ks < kKeys / 16; ++ks) mmaTS(tmem + kColO + t * D, tmem + kColS + t * kKeys + 8 * ks, v + ks * (16 * 128 >> 4), idescO, ks > 0 || more ? 1u : 0u);
+      };
+      uint32_t slot = 0, phase = 0;                   // the next item's slot, and the parity of its load
+      auto step = [&]() { if (++slot == C::kSlots) { slot = 0; phase ^= 1u; } };
+      uint32_t ph0 = 0, ph1 = 0;                      // parities of the tiles' weights
+      bool more0 = false, more1 = false;              // a tile's sums have been started
       if (begin < end) {
-        slotWait(0);
+        ok = ok && waitAt(full, 0, gone);
         tcFenceAfter();
-        for (int t = 0; t < 2; ++t) if (active(t, begin)) issueS(t, 0);
-        mmaCommit(&kvEmpty[0]);
+        if (active(n0, begin)) issueS(0, 0);
+        if (active(n1, begin)) issueS(1, 0);
+        commitAt(empty);
+        step();
       }
       for (int u = begin; u < end; ++u) {
-        const uint32_t vItem = 2 * (u - begin) + 1, kItem = vItem + 1;
-        bool haveV = false, haveK = false;
-        for (int t = 0; t < 2; ++t) {
-          if (active(t, u)) {
-            if (!haveV) { slotWait(vItem); haveV = true; }
-            ok = ok && mbarWait(&pReady[t], weights[t] & 1u, abortWord);
-            ++weights[t];
-            tcFenceAfter();
-            const uint32_t v = smemAddr(ring + (vItem % C::kSlots) * C::kTile);
-#pragma unroll
-            for (int ks = 0; ks < kKeys / 16; ++ks)
-              mmaTS(tmem + kColO + t * D, tmem + kColS + t * kKeys + 8 * ks, smemDescMnMajorSw128(v + ks * 16 * 128, C::kAtom), idescO, ks > 0 || started[t] ? 1u : 0u);
-            started[t] = true;
-          }
-          if (u + 1 < end && active(t, u + 1)) {
-            if (!haveK) { slotWait(kItem); haveK = true; tcFenceAfter(); }
-            issueS(t, kItem);
-          }
+        const uint32_t vSlot = slot;
+        ok = ok && waitAt(full + 8 * slot, phase, gone);
+        step();
+        const uint32_t kSlot = slot, kPhase = phase;
+        const bool next = u + 1 < end;
+        bool haveK = false;
+        if (active(n0, u)) {
+          ok = ok && waitAt(pr, ph0, gone);
+          ph0 ^= 1u;
+          tcFenceAfter();
+          issueO(0, vSlot, more0);
+          more0 = true;
         }
-        if (!haveV) slotWait(vItem);                  // a slot is given back only after its load has landed
-        mmaCommit(&kvEmpty[vItem % C::kSlots]);
-        if (u + 1 < end) {
-          if (!haveK) slotWait(kItem);
-          mmaCommit(&kvEmpty[kItem % C::kSlots]);
+        if (next && active(n0, u + 1)) {
+          ok = ok && waitAt(full + 8 * kSlot, kPhase, gone);
+          haveK = true;
+          tcFenceAfter();
+          issueS(0, kSlot);
+        }
+        if (active(n1, u)) {
+          ok = ok && waitAt(pr + 8, ph1, gone);
+          ph1 ^= 1u;
+          tcFenceAfter();
+          issueO(1, vSlot, more1);
+          more1 = true;
+        }
+        commitAt(empty + 8 * vSlot);
+        if (next) {
+          if (!haveK) { ok = ok && waitAt(full + 8 * kSlot, kPhase, gone); tcFenceAfter(); }   // a slot is given back only after its load has landed
+          if (active(n1, u + 1)) issueS(1, kSlot);
+          commitAt(empty + 8 * kSlot);
+          step();
         }
       }
       mmaCommit(&oFull[0]);
@@ -263,24 +362,29 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     }
   } else {
     // ------------------------------------------------------------------ softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int t = warp >> 2, r = threadIdx.x & 127, q4 = warp & 3;
-    const Tile tile = t ? tile1 : tile0;
-    const long long row = row0 + t * kTileRows + r;
-    const bool live = row < rows;
-    const long long tok = (live ? row : rows - 1) / p.group;
-    const long long pos = s.len - s.n + tok;
-    const int head = h * p.group + (int)((live ? row : rows - 1) - tok * p.group);
-    const long long qOff = (s.begin + tok) * p.qSt + head * p.qSh, oOff = (s.begin + tok) * p.oSt + head * p.oSh;
+    const int t = warp >> 3, side = (warp >> 2) & 1, q4 = warp & 3, r = q4 * 32 + lane;   // tile, half of the columns, row
+    // this thread's row: its place, and where it lies in q and out (worked out again after the loop)
+    auto liveRow = [&]() { return plan->row0 + t * kTileRows + r < plan->rows; };
+    auto offsetOf = [&](long long sTok, long long sHead) {
+      const long long row = plan->row0 + t * kTileRows + r, x = row < plan->rows ? row : plan->rows - 1, tok = x / p.group;
+      return (plan->qBegin + tok) * sTok + (h * p.group + (x - tok * p.group)) * sHead;
+    };
+    const long long row = plan->row0 + t * kTileRows + r;
+    const int pos = clipPlace((long long)plan->len - plan->n + (row < plan->rows ? row : plan->rows - 1) / p.group);
     uint8_t* tileQ = sQ + t * C::kTile;
+    const uint32_t mineAt = smemAddr(sRow + (t * 2 + side) * kTileRows + r), otherAt = smemAddr(sRow + (t * 2 + (side ^ 1)) * kTileRows + r);
+    const int bar = 1 + t * 4 + q4;                   // the two warps that share 32 rows
     constexpr int kChunks = D / 8;                    // 16-byte chunks of a row
     constexpr int kRowsAtOnce = 32 / kChunks;         // rows that a warp's 16-byte accesses cover
-    // Q, a warp its own 32 rows: neighbouring lanes take neighbouring chunks of a row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const long long qOff = offsetOf(p.qSt, p.qSh);
+    const bool inQ = liveRow();
+    // Q, a warp 16 of its 32 rows: neighbouring lanes take neighbouring chunks of a row
 #pragma unroll 4
-    for (int i = 0; i < 32; i += kRowsAtOnce) {
-      const int src = i + lane / kChunks, c = lane % kChunks, rr = q4 * 32 + src;
+    for (int i = 0; i < 16; i += kRowsAtOnce) {
+      const int src = side * 16 + i + lane / kChunks, c = lane % kChunks, rr = q4 * 32 + src;
       const long long off = __shfl_sync(0xffffffffu, qOff, src);
-      const bool in = __shfl_sync(0xffffffffu, (int)live, src);
+      const bool in = __shfl_sync(0xffffffffu, (int)inQ, src);
       uint4 x = make_uint4(0, 0, 0, 0);
       if (in) x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + off + c * 8);
       if (a.signQ < 0.f) { x.x ^= 0x80008000u; x.y ^= 0x80008000u; x.z ^= 0x80008000u; x.w ^= 0x80008000u; }
@@ -291,108 +395,124 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     if (lane == 0) mbarArrive(qReady);
 
     const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
-    const uint32_t colS = tmem + lanes + kColS + t * kKeys, colO = tmem + lanes + kColO + t * D;
+    const uint32_t colS = tmem + lanes + kColS + t * kKeys, colO = tmem + lanes + kColO + t * D + side * (D / 2);
     constexpr float kShift = weightShift<T>();
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;                     // the row's running maximum (the same in both threads), this thread's share of the sum
     uint32_t done = 0;                                // blocks of this tile so far
     bool ok = true;
-    for (int u = begin; u < end; ++u) {
-      const long long j0 = keyOf(bl, u, kKeys);
-      if (!tile.active(j0)) continue;
-      if (ok && !mbarWait(&sFull[t], done & 1u, abortWord)) { ok = false; atomicExch(&g_pagedChunkStatus, 12); }
+    const int end = plan->end;
+    const uint32_t fullAt = smemAddr(&sFull[t]), readyAt = smemAddr(&pReady[t]), gone = smemAddr((const void*)abortWord);
+    for (int u = plan->begin; u < end; ++u) {
+      const Units n = plan->units[t];
+      if (u >= n.sink && u < n.lo) { u = n.lo - 1; continue; }
+      if (u >= n.hi && u >= n.sink) break;
+      if (ok && !waitAt(fullAt, done & 1u, gone)) { ok = false; atomicExch(&g_pagedChunkStatus, 12); }
       tcFenceAfter();
       __syncwarp();
-      uint32_t x[4][32];
+      uint32_t x[2][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmemIssue32(colS + 32 * c, x[c]);
+      for (int c = 0; c < 2; ++c) tmemIssue32(colS + side * 64 + 32 * c, x[c]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmemWait32(x[c]);
-      // every row sees all keys: they lie before the tile's first token, and inside its last one's window or among the sinks
-      const bool whole = j0 + kKeys - 1 <= tile.first && (j0 > tile.last - p.window || j0 + kKeys <= p.sinks);
+      for (int c = 0; c < 2; ++c) tmemWait32(x[c]);
+      const bool whole = u < n.wholeSink || (u >= n.wholeLo && u < n.wholeHi);
       if (!whole) {
-        // visible columns: c <= hi and (c >= lo or c < sink)
-        const long long hi64 = pos - j0, lo64 = pos - p.window + 1 - j0, sink64 = p.sinks - j0;
-        const int hi = hi64 > kKeys ? kKeys : hi64 < -1 ? -1 : (int)hi64, lo = lo64 < 0 ? 0 : lo64 > kKeys ? kKeys : (int)lo64;
-        const int sink = sink64 < 0 ? 0 : sink64 > kKeys ? kKeys : (int)sink64;
+        // visible columns: c < hi and (c >= lo or c < sink), as bits (a branch a column costs 8 us a block)
+        const int j1 = keyOf(plan->bl, u, kKeys) + side * 64, hi = pos + 1 - j1, lo = max(pos + 1 - p.window, 0) - j1, sink = p.sinks - j1;
 #pragma unroll
-        for (int c = 0; c < kKeys; ++c)
-          if (!(c <= hi && (c >= lo || c < sink))) x[c >> 5][c & 31] = 0xff800000u;   // -inf, whatever the score is
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t vis = bitsBelow(hi - 32 * c) & (~bitsBelow(lo - 32 * c) | bitsBelow(sink - 32 * c));
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[c][i] = (vis >> i) & 1u ? x[c][i] : 0xff800000u;   // -inf, whatever the score is
+        }
       }
       float mx[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(x[c][0]);
+        mx[c] = __uint_as_float(x[c >> 1][16 * (c & 1)]);
 #pragma unroll
-        for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(x[c][i]));
+        for (int i = 1; i < 16; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(x[c >> 1][16 * (c & 1) + i]));
       }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scaleAbs;
+      float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scaleAbs;
+      // The two warps meet: both have taken their scores out of tensor memory (the weights will lie over them), and both know whether some
+      // row's maximum has to move.
       float keep = 1.f;
-      if (top > m + kRescaleStep) { keep = exp2Fast(m - top); m = top; }
-      const float base = m == -INFINITY ? 0.f : m - kShift;
-      l *= keep;
-      if (done > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
-        // some row of the warp moved its maximum; the scores' barrier says that all products into O are complete
+      if (barrierOr(bar, top > m + kRescaleStep)) {
+        storeShared(mineAt, top);
+        pairBarrier(bar);
+        top = fmaxf(top, loadShared(otherAt));
+        if (top > m + kRescaleStep) { keep = exp2Fast(m - top); m = top; l *= keep; }
+        if (done > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
+          // the scores' barrier says that all products into O are complete
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          float o[32];
-          tmemLoad32x32(colO + c, o);
+          for (int c = 0; c < D / 2; c += 32) {
+            float o[32];
+            tmemLoad32x32(colO + c, o);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] *= keep;
-          tmemStore32(colO + c, reinterpret_cast<uint32_t*>(o));
-          tmemStoreWait();
+            for (int i = 0; i < 32; ++i) o[i] *= keep;
+            tmemStore32(colO + c, reinterpret_cast<uint32_t*>(o));
+            tmemStoreWait();
+          }
         }
+        pairBarrier(bar);                             // both have read the other's maximum
       }
+      const float base = m == -INFINITY ? 0.f : m - kShift;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t w[32];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int c = half * 64 + 2 * i;
-          float y0 = __uint_as_float(x[c >> 5][c & 31]), y1 = __uint_as_float(x[c >> 5][(c & 31) + 1]);
-          fma2(y0, y1, a.scaleAbs, a.scaleAbs, -base, -base);
-          y0 = exp2Fast(y0); y1 = exp2Fast(y1);
-          sum[(i & 1) * 2] += y0; sum[(i & 1) * 2 + 1] += y1;
-          w[i] = pack2<T>(y0, y1);
-        }
-        __syncwarp();
-        tmemStore32(colS + 32 * half, w);
+      for (int i = 0; i < 32; ++i) {
+        float y0 = __uint_as_float(x[i >> 4][2 * i & 31]), y1 = __uint_as_float(x[i >> 4][(2 * i & 31) + 1]);
+        fma2(y0, y1, a.scaleAbs, a.scaleAbs, -base, -base);
+        y0 = exp2Fast(y0); y1 = exp2Fast(y1);
+        add2(sum[(i & 1) * 2], sum[(i & 1) * 2 + 1], y0, y1);
+        w[i] = pack2<T>(y0, y1);
       }
+      __syncwarp();
+      tmemStore32(colS + 32 * side, w);
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmemStoreWait();
-      // Values of keys that no row sees may be NaN, and 0 x NaN is NaN: the tile that uses the block first zeroes them, thread r key r.
-      const bool clean = j0 + kKeys <= seen.sinkEnd || (j0 + kKeys <= seen.hi && (j0 >= seen.lo || seen.sinkEnd == seen.lo));
-      if (!clean && (t == 0 || !tile0.active(j0))) {
-        const uint32_t vItem = 2 * (u - begin) + 1;
-        if (ok && !mbarWait(&kvFull[vItem % C::kSlots], (vItem / C::kSlots) & 1u, abortWord)) { ok = false; atomicExch(&g_pagedChunkStatus, 12); }
-        const long long j = j0 + r;
-        if (!(j < seen.sinkEnd || (j >= seen.lo && j < seen.hi))) {
+      if (!whole) {
+        // Values of keys that no row sees may be NaN, and 0 x NaN is NaN: the tile that uses the block first zeroes them, row r key r.
+        const Seen seen = plan->seen;
+        const Units n0 = plan->units[0];
+        const int j0 = keyOf(plan->bl, u, kKeys), j = j0 + r;
+        const bool clean = j0 + kKeys <= seen.sinkEnd || (j0 + kKeys <= seen.hi && (j0 >= seen.lo || seen.sinkEnd == seen.lo));
+        if (!clean && (t == 0 || !(u < n0.sink || (u >= n0.lo && u < n0.hi)))) {
+          const uint32_t vItem = 2 * (u - plan->begin) + 1;
+          if (ok && !waitAt(smemAddr(&kvFull[vItem % C::kSlots]), (vItem / C::kSlots) & 1u, gone)) { ok = false; atomicExch(&g_pagedChunkStatus, 12); }
+          if (!(j < seen.sinkEnd || (j >= seen.lo && j < seen.hi))) {
 #pragma unroll
-          for (int i = 0; i < kChunks; ++i) *reinterpret_cast<uint4*>(ring + (vItem % C::kSlots) * C::kTile + (i >> 3) * C::kAtom + r * 128 + ((i & 7) << 4)) = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < kChunks / 2; ++i) {
+              const int c = side * (kChunks / 2) + ((i + r) & (kChunks / 2 - 1));   // neighbouring rows start at other banks
+              *reinterpret_cast<uint4*>(ring + (vItem % C::kSlots) * C::kTile + (c >> 3) * C::kAtom + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          fenceProxyAsync();
         }
-        fenceProxyAsync();
       }
       tcFenceBefore();
       __syncwarp();
-      if (lane == 0) mbarArrive(&pReady[t]);
+      if (lane == 0) arriveAt(readyAt);
       ++done;
     }
     // ---------------------------------------------------------------- output
+    storeShared(mineAt, l);
     if (ok && !mbarWait(&oFull[t], 0, abortWord)) { ok = false; atomicExch(&g_pagedChunkStatus, 12); }
     tcFenceAfter();
-    __syncwarp();
+    pairBarrier(bar);
+    l += loadShared(otherAt);
     const float base = m == -INFINITY ? 0.f : m - kShift;
     const bool cut = a.splits > 1;
     float* part = a.parts + ((pair * 2 + t) * a.splits + split) * C::kPart;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     bool odd = false;
-    if (cut) {
+    if (cut && side == 0) {
       part[kTileRows * D + r] = m;
       part[kTileRows * (D + 1) + r] = l;
     }
 #pragma unroll 1
-    for (int c = 0; c < D; c += 32) {
+    for (int c = 0; c < D / 2; c += 32) {
       float o[32];
+      __syncwarp();
       if (done) tmemLoad32x32(colO + c, o);
       else {
 #pragma unroll
@@ -400,27 +520,30 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
       }
 #pragma unroll
       for (int i = 0; i < 32; ++i) odd = odd || !(fabsf(o[i]) <= 3.402823466e38f);
+      const int col = side * (D / 2) + c;
       if (cut) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<float4*>(part + ((long long)(c / 4 + i) * kTileRows + r) * 4) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          *reinterpret_cast<float4*>(part + ((long long)(col / 4 + i) * kTileRows + r) * 4) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int ch = c / 8 + i;
+          const int ch = col / 8 + i;
           *reinterpret_cast<uint4*>(tileQ + (ch >> 3) * C::kAtom + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) =
               make_uint4(pack2<T>(o[8 * i] * inv, o[8 * i + 1] * inv), pack2<T>(o[8 * i + 2] * inv, o[8 * i + 3] * inv), pack2<T>(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
                          pack2<T>(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
         }
       }
     }
-    __syncwarp();
+    pairBarrier(bar);
+    const bool live = liveRow();
+    const long long qAt = offsetOf(p.qSt, p.qSh), oOff = offsetOf(p.oSt, p.oSh);
     unsigned redo = __ballot_sync(0xffffffffu, odd && live && fabsf(l) <= 3.402823466e38f);
     while (redo) {
       const int src = __ffs(redo) - 1, rr = q4 * 32 + src;
       redo &= redo - 1;
       float o[D / 32];
-      sumRow<T, D>(a, b, h, __shfl_sync(0xffffffffu, qOff, src), __shfl_sync(0xffffffffu, pos, src), bl, begin, end, __shfl_sync(0xffffffffu, base, src), o);
+      sumRow<T, D>(a, plan->seq, h, __shfl_sync(0xffffffffu, qAt, src), __shfl_sync(0xffffffffu, pos, src), plan->bl, plan->begin, plan->end, __shfl_sync(0xffffffffu, base, src), o);
       const float f = __shfl_sync(0xffffffffu, inv, src);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
@@ -433,11 +556,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
         }
       }
     }
-    __syncwarp();
+    pairBarrier(bar);
     if (!cut) {
 #pragma unroll 4
-      for (int i = 0; i < 32; i += kRowsAtOnce) {
-        const int src = i + lane / kChunks, c = lane % kChunks, rr = q4 * 32 + src;
+      for (int i = 0; i < 16; i += kRowsAtOnce) {
+        const int src = side * 16 + i + lane / kChunks, c = lane % kChunks, rr = q4 * 32 + src;
         const long long off = __shfl_sync(0xffffffffu, oOff, src);
         const bool in = __shfl_sync(0xffffffffu, (int)live, src);
         const uint4 x = *reinterpret_cast<const uint4*>(tileQ + (c >> 3) * C::kAtom + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
@@ -447,7 +570,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
   }
   tcFenceBefore();
   __syncthreads();
-  if (warp == 9) { tcFenceAfter(); tmemDealloc(tmem, 512); }
+  if (warp == kIssuerWarp) { tcFenceAfter(); tmemDealloc(tmem, 512); }
 }
 
 // Joins the parts of a tile: block = one tile of 128 rows, thread = one row and every other vector of four elements.
@@ -462,7 +585,7 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const ChunkArgs a
   const int4 rec = a.records[pair];
   if (rec.x < 0) return;
   const Sequence s = sequenceOf(p, rec.x);
-  const long long rows = s.n * p.group, row = (long long)rec.y * kCtaRows + t * kTileRows + r;
+  const long long rows = (long long)s.n * p.group, row = (long long)rec.y * kCtaRows + t * kTileRows + r;
   const float* part = a.parts + (pair * 2 + t) * a.splits * C::kPart;
   float top = -INFINITY, sum = 0.f;
   for (int i = 0; i < a.splits; ++i) top = fmaxf(top, part[(long long)i * C::kPart + kTileRows * D + r]);
@@ -501,7 +624,7 @@ Launch launchOf(const PagedArgs& p) {
   l.tiles = each * p.batch < most ? each * p.batch : most;
   const long long ctas = l.tiles * p.kvHeads, sms = deviceSMs();
   long long longest = p.reach;
-  if (p.window + p.sinks + kCtaRows < longest) longest = p.window + p.sinks + kCtaRows;
+  if ((long long)p.window + p.sinks + kCtaRows < longest) longest = (long long)p.window + p.sinks + kCtaRows;
   long long splits = ctas >= sms ? 1 : sms / ctas;
   const long long most2 = (longest + 2 * kKeys - 1) / (2 * kKeys);
   if (splits > most2) splits = most2;

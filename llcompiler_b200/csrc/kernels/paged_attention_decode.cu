@@ -51,14 +51,14 @@ struct DecodeArgs {
 // The blocks of keys of one key head of a sequence; one empty block where nothing is visible, which writes the zeros; none where the
 // sequence has no rows, or more than this kernel takes.
 __device__ __forceinline__ Blocks blocksOf(const PagedArgs& p, const Sequence& s, const Seen& seen, int maxRows) {
-  if (s.n == 0 || s.n * p.group > maxRows) return Blocks{0, 0, 0};
+  if (s.n == 0 || (long long)s.n * p.group > maxRows) return Blocks{0, 0, 0};
   Blocks b = blocksOf(seen, kKeys);
   if (b.count < 1) b.count = 1;
   return b;
 }
 __device__ __forceinline__ int countOf(const PagedArgs& p, int b, int maxRows) {
   const Sequence s = sequenceOf(p, b);
-  return blocksOf(p, s, seenBy(p, s.len - s.n, s.len - 1), maxRows).count;
+  return blocksOf(p, s, seenBy(p, clipPlace((long long)s.len - s.n), s.len - 1), maxRows).count;
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t* r) {
@@ -166,14 +166,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
     const int box = lane % boxes, half = lane / boxes % (D / 64), which = lane / (boxes * (D / 64));   // this lane's load of every stage
     while (left > 0 && ok) {
       const Sequence s = sequenceOf(p, b);
-      const Seen seen = seenBy(p, s.len - s.n, s.len - 1);
+      const Seen seen = seenBy(p, clipPlace((long long)s.len - s.n), s.len - 1);
       const Blocks bl = blocksOf(p, s, seen, C::kRows);
       if (bl.count == 0) { ++b; h = 0; continue; }
       const long long end = unit + left < bl.count ? unit + left : bl.count;
       left -= end - unit;
       for (; unit < end && ok; ++unit, ++it) {
         const int st = it % C::kStages;
-        const long long j = keyOf(bl, unit, kKeys) + (long long)box * a.boxRows;
+        const long long j = keyOf(bl, (int)unit, kKeys) + (long long)box * a.boxRows;
         // a box that no token sees any key of is not looked up: it reads as zeros, as does one with a bad page number
         const bool wanted = lane < loads && (j < seen.sinkEnd || (j < seen.hi && j + a.boxRows > seen.lo));
         long long page = -1;
@@ -211,7 +211,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
   int4 record = make_int4(-1, 0, 0, 0);
   while (left > 0) {
     const Sequence s = sequenceOf(p, b);
-    const Seen seen = seenBy(p, s.len - s.n, s.len - 1);
+    const Seen seen = seenBy(p, clipPlace((long long)s.len - s.n), s.len - 1);
     const Blocks bl = blocksOf(p, s, seen, C::kRows);
     if (bl.count == 0) { ++b; h = 0; continue; }
     const long long begin = unit, end = unit + left < bl.count ? unit + left : bl.count;
@@ -244,7 +244,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
     }
     for (; unit < end; ++unit, ++it) {
       const int st = it % C::kStages;
-      const long long j0 = keyOf(bl, unit, kKeys) + warp * 16;   // this warp's keys
+      const long long j0 = keyOf(bl, (int)unit, kKeys) + warp * 16;   // this warp's keys
       if (ok && !mbarWait(&full[st], (it / C::kStages) & 1u, abortWord)) { ok = false; atomicExch(&g_pagedDecodeStatus, 9); }
       __syncwarp();
       const uint32_t kAddr = kBase + st * C::kStage, vAddr = vBase + st * C::kStage;
@@ -473,7 +473,7 @@ struct Launch { bool split; unsigned ctas; };
 template <int D, int MT> Launch launchOf(const PagedArgs& p) {
   const long long pairs = (long long)p.batch * p.kvHeads;
   long long longest = p.reach;                     // keys that a sequence can see
-  if (p.window + p.sinks + MT * 16 < longest) longest = p.window + p.sinks + MT * 16;
+  if ((long long)p.window + p.sinks + MT * 16 < longest) longest = (long long)p.window + p.sinks + MT * 16;
   const long long slots = (long long)Config<D, MT>::kCtas * deviceSMs();
   // up to 512 keys a pair the second launch costs more than a cut saves
   if (longest <= 512) return {false, (unsigned)pairs};

@@ -142,6 +142,10 @@ __device__ __forceinline__ void fma2(float& x0, float& x1, float s0, float s1, f
       "fma.rn.f32x2 x, x, s, b;\n\tmov.b64 {%0, %1}, x;\n\t}"
       : "+f"(x0), "+f"(x1) : "f"(s0), "f"(s1), "f"(b0), "f"(b1));
 }
+// (x0, x1) += (y0, y1) in one instruction.
+__device__ __forceinline__ void add2(float& x0, float& x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+f"(x0), "+f"(x1) : "f"(y0), "f"(y1));
+}
 // geluTanhBf16 (common.cuh) of two values, the same operations on packed pairs.
 __device__ __forceinline__ void geluTanhBf16x2(float& x0, float& x1) {
   float u0, u1, h0, h1;
