@@ -81,6 +81,15 @@ __device__ __forceinline__ Units unitsOf(const PagedArgs& p, const Tile& t, cons
   return n;
 }
 
+// The same value in every lane, known as such to the compiler.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ Units uniform(const Units& n) { return Units{uniform(n.sink), uniform(n.lo), uniform(n.hi), uniform(n.wholeSink), uniform(n.wholeLo), uniform(n.wholeHi)}; }
+__device__ __forceinline__ bool electOne() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
+}
+
 // What a CTA does, worked out by one thread and read from shared memory where it is needed: kept in registers it would displace scores.
 struct Plan {
   Units units[2];              // of the two tiles
@@ -180,7 +189,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
   Plan* plan = reinterpret_cast<Plan*>(misc + 512);
   float* sRow = reinterpret_cast<float*>(misc + 1024);           // [2 tiles][2 halves][128]
   const PagedArgs& p = a.p;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (smemAddr(smem) & 1023) {                        // the swizzled tiles need it; no static shared memory lies before them
     if (threadIdx.x == 0) {
       atomicExch(&g_pagedChunkStatus, 10);
@@ -285,13 +294,17 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
         if (lane == 0) atomicExch(&g_pagedChunkStatus, 10);
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);   // copies in flight land before the CTA gives its memory back
       }
-    } else if (warp == kIssuerWarp && lane == 0) {
+    } else if (warp == kIssuerWarp) {
       // ---------------------------------------------------------------- issuer
-      // One thread feeds the tensor pipe: descriptors are built once, a slot only adds its offset, and the loop has no division.
+      // The whole warp walks the loop, one elected thread issues: what the products are given then stays in uniform registers (a loop
+      // run by one thread alone moved every descriptor there anew, 90 cycles a product of 64).  Descriptors are built once, a slot only
+      // adds its offset, and the loop has no division.
       constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
       constexpr uint32_t idescS = instrDesc(fmt, kTileRows, kKeys, 0, 0), idescO = instrDesc(fmt, kTileRows, D, 0, 1);
-      const Units n0 = plan->units[0], n1 = plan->units[1];
-      const int begin = plan->begin, end = plan->end;
+      const Units n0 = uniform(plan->units[0]), n1 = uniform(plan->units[1]);
+      const int begin = uniform(plan->begin), end = uniform(plan->end);
+      const uint32_t tm = uniform((int)tmem);
+      const bool leader = electOne();
       const uint64_t descQ = smemDescKMajorSw128(smemAddr(sQ)), descK = smemDescKMajorSw128(smemAddr(ring)), descV = smemDescMnMajorSw128(smemAddr(ring), C::kAtom);
       const uint32_t full = smemAddr(kvFull), empty = smemAddr(kvEmpty), sf = smemAddr(sFull), pr = smemAddr(pReady), gone = smemAddr((const void*)abortWord);
       constexpr uint32_t kAtom16 = C::kAtom >> 4, kTile16 = C::kTile >> 4;
@@ -299,15 +312,17 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
       auto active = [&](const Units& n, int u) { return u < n.sink || (u >= n.lo && u < n.hi); };
       auto issueS = [&](int t, uint32_t slot) {
         const uint64_t q = descQ + t * kTile16, k = descK + slot * kTile16;
+        if (!leader) return;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
-          mmaSS<false>(tmem + kColS + t * kKeys, q + (ks / 4) * kAtom16 + 2 * (ks % 4), k + (ks / 4) * kAtom16 + 2 * (ks % 4), idescS, ks > 0 ? 1u : 0u);
+          mmaSS<false>(tm + kColS + t * kKeys, q + (ks / 4) * kAtom16 + 2 * (ks % 4), k + (ks / 4) * kAtom16 + 2 * (ks % 4), idescS, ks > 0 ? 1u : 0u);
         commitAt(sf + 8 * t);
       };
       auto issueO = [&](int t, uint32_t slot, bool more) {
         const uint64_t v = descV + slot * kTile16;
+        if (!leader) return;
 #pragma unroll
-        for (int ks = 0; ks < kKeys / 16; ++ks) mmaTS(tmem + kColO + t * D, tmem + kColS + t * kKeys + 8 * ks, v + ks * (16 * 128 >> 4), idescO, ks > 0 || more ? 1u : 0u);
+        for (int ks = 0; ks < kKeys / 16; ++ks) mmaTS(tm + kColO + t * D, tm + kColS + t * kKeys + 8 * ks, v + ks * (16 * 128 >> 4), idescO, ks > 0 || more ? 1u : 0u);
       };
       uint32_t slot = 0, phase = 0;                   // the next item's slot, and the parity of its load
       auto step = [&]() { if (++slot == C::kSlots) { slot = 0; phase ^= 1u; } };
@@ -318,7 +333,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
         tcFenceAfter();
         if (active(n0, begin)) issueS(0, 0);
         if (active(n1, begin)) issueS(1, 0);
-        commitAt(empty);
+        if (leader) commitAt(empty);
         step();
       }
       for (int u = begin; u < end; ++u) {
@@ -348,17 +363,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
           issueO(1, vSlot, more1);
           more1 = true;
         }
-        commitAt(empty + 8 * vSlot);
+        if (leader) commitAt(empty + 8 * vSlot);
         if (next) {
           if (!haveK) { ok = ok && waitAt(full + 8 * kSlot, kPhase, gone); tcFenceAfter(); }   // a slot is given back only after its load has landed
           if (active(n1, u + 1)) issueS(1, kSlot);
-          commitAt(empty + 8 * kSlot);
+          if (leader) commitAt(empty + 8 * kSlot);
           step();
         }
       }
-      mmaCommit(&oFull[0]);
-      mmaCommit(&oFull[1]);
-      if (!ok) atomicExch(&g_pagedChunkStatus, 11);
+      if (leader) { commitAt(smemAddr(&oFull[0])); commitAt(smemAddr(&oFull[1])); }
+      if (!ok && leader) atomicExch(&g_pagedChunkStatus, 11);
     }
   } else {
     // ------------------------------------------------------------------ softmax
