@@ -130,6 +130,37 @@ __device__ __forceinline__ long long tilesOf(const PagedArgs& p, int b, int done
   return rows <= doneRows ? 0 : (rows + kCtaRows - 1) / kCtaRows;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+// 2^x of two numbers without the special-function unit, which computes 16 a cycle and SM and would be what a block waits for: x = n + r with
+// n the nearest whole number and |r| <= 1/2, 2^r by a polynomial (the least maximal relative error of its degree: 2^-13.7 for bf16, whose
+// weights are rounded to 2^-9 right after, 2^-18.5 for f16), 2^n by its exponent bits.  Below -126 the result is 2^-126, NaN stays NaN.
+constexpr int kPolyOf4 = 1;               // of 4 pairs, in blocks that every row sees whole
+template <typename T> __device__ __forceinline__ void exp2Poly2(float& x0, float& x1) {
+  constexpr float kRound = 12582912.f + 127.f;        // 1.5 x 2^23: the sum's last bits are n + 127
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-126.f));
+  float t0 = x0, t1 = x1;
+  add2(t0, t1, kRound, kRound);
+  float n0 = t0, n1 = t1;
+  add2(n0, n1, -kRound, -kRound);
+  fma2(n0, n1, -1.f, -1.f, x0, x1);                   // r = x - n
+  float p0, p1;
+  if constexpr (std::is_same<T, __half>::value) {
+    p0 = p1 = 0.009570102207362652f;
+    horner2(p0, p1, n0, n1, 0.05591785907745361f);
+    horner2(p0, p1, n0, n1, 0.240247443318367f);
+    horner2(p0, p1, n0, n1, 0.6931217908859253f);
+    horner2(p0, p1, n0, n1, 0.9999992847442627f);
+  } else {
+    p0 = p1 = 0.0551716685295105f;
+    horner2(p0, p1, n0, n1, 0.2426111251115799f);
+    horner2(p0, p1, n0, n1, 0.6932609677314758f);
+    horner2(p0, p1, n0, n1, 0.9999280571937561f);
+  }
+  x0 = p0 * __uint_as_float(__float_as_uint(t0) << 23);
+  x1 = p1 * __uint_as_float(__float_as_uint(t1) << 23);
+}
+
 // Barriers of the two warps that share 32 rows; the first also tells whether any of the 64 threads said yes.
 __device__ __forceinline__ void pairBarrier(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ bool barrierOr(int id, bool yes) {
@@ -422,38 +453,67 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
       if (u >= n.hi && u >= n.sink) break;
       if (ok && !waitAt(fullAt, done & 1u, gone)) { ok = false; atomicExch(&g_pagedChunkStatus, 12); }
       tcFenceAfter();
-      __syncwarp();
-      uint32_t x[2][32];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) tmemIssue32(colS + side * 64 + 32 * c, x[c]);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) tmemWait32(x[c]);
       const bool whole = u < n.wholeSink || (u >= n.wholeLo && u < n.wholeHi);
-      if (!whole) {
-        // visible columns: c < hi and (c >= lo or c < sink), as bits (a branch a column costs 8 us a block)
-        const int j1 = keyOf(plan->bl, u, kKeys) + side * 64, hi = pos + 1 - j1, lo = max(pos + 1 - p.window, 0) - j1, sink = p.sinks - j1;
+      uint32_t x[64], w[32];
+      auto load = [&]() {
+        __syncwarp();
+        tmemIssue32(colS + side * 64, x);
+        tmemIssue32(colS + side * 64 + 32, x + 32);
+        tmemWait32(x);
+        tmemWait32(x + 32);
+        if (!whole) {
+          // visible columns: c < hi and (c >= lo or c < sink), as bits (a branch a column costs 8 us a block)
+          const int j1 = keyOf(plan->bl, u, kKeys) + side * 64, hi = pos + 1 - j1, lo = max(pos + 1 - p.window, 0) - j1, sink = p.sinks - j1;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t vis = bitsBelow(hi - 32 * c) & (~bitsBelow(lo - 32 * c) | bitsBelow(sink - 32 * c));
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t vis = bitsBelow(hi - 32 * c) & (~bitsBelow(lo - 32 * c) | bitsBelow(sink - 32 * c));
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[c][i] = (vis >> i) & 1u ? x[c][i] : 0xff800000u;   // -inf, whatever the score is
+            for (int i = 0; i < 32; ++i) x[32 * c + i] = (vis >> i) & 1u ? x[32 * c + i] : 0xff800000u;   // -inf, whatever the score is
+          }
         }
-      }
-      float mx[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(x[c >> 1][16 * (c & 1)]);
-#pragma unroll
-        for (int i = 1; i < 16; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(x[c >> 1][16 * (c & 1) + i]));
-      }
-      float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scaleAbs;
-      // The two warps meet: both have taken their scores out of tensor memory (the weights will lie over them), and both know whether some
-      // row's maximum has to move.
-      float keep = 1.f;
-      if (barrierOr(bar, top > m + kRescaleStep)) {
-        storeShared(mineAt, top);
+      };
+      // The row's largest score of this block, from both its threads.
+      auto exchange = [&](float mine) {
+        storeShared(mineAt, mine);
         pairBarrier(bar);
-        top = fmaxf(top, loadShared(otherAt));
+        return fmaxf(mine, loadShared(otherAt));
+      };
+      if (done == 0) {                                // the first block sets the maximum before its weights are taken
+        load();
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mx[i & 3] = max3(mx[i & 3], __uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+        m = exchange(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scaleAbs);
+      }
+      // Weights relative to the maximum so far, and the block's own maximum beside them: no exponential waits for it.  If some row's grew by
+      // more than the step, the block is taken again from tensor memory (the weights have not been stored over it yet).
+      for (;;) {
+        load();
+        const float base = m == -INFINITY ? 0.f : m - kShift;
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+        auto weights = [&](auto poly) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float y0 = __uint_as_float(x[2 * i]), y1 = __uint_as_float(x[2 * i + 1]);
+            mx[i & 3] = max3(mx[i & 3], y0, y1);
+            fma2(y0, y1, a.scaleAbs, a.scaleAbs, -base, -base);
+            if (decltype(poly)::value && i % 4 >= 4 - kPolyOf4) exp2Poly2<T>(y0, y1);
+            else { y0 = exp2Fast(y0); y1 = exp2Fast(y1); }
+            add2(sum[(i & 1) * 2], sum[(i & 1) * 2 + 1], y0, y1);
+            w[i] = pack2<T>(y0, y1);
+          }
+        };
+        // two loops: with the choice inside, every pair of weights is a branch
+        if (whole) weights(std::true_type{});
+        else weights(std::false_type{});
+        const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scaleAbs;
+        // The row's two warps meet here in any case: both have taken their scores out before either stores weights over them.
+        if (!barrierOr(bar, mine > m + kRescaleStep)) {
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          break;
+        }
+        const float top = exchange(mine);
+        float keep = 1.f;
         if (top > m + kRescaleStep) { keep = exp2Fast(m - top); m = top; l *= keep; }
         if (done > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
           // the scores' barrier says that all products into O are complete
@@ -467,22 +527,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
             tmemStoreWait();
           }
         }
-        pairBarrier(bar);                             // both have read the other's maximum
-      }
-      const float base = m == -INFINITY ? 0.f : m - kShift;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-      uint32_t w[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        float y0 = __uint_as_float(x[i >> 4][2 * i & 31]), y1 = __uint_as_float(x[i >> 4][(2 * i & 31) + 1]);
-        fma2(y0, y1, a.scaleAbs, a.scaleAbs, -base, -base);
-        y0 = exp2Fast(y0); y1 = exp2Fast(y1);
-        add2(sum[(i & 1) * 2], sum[(i & 1) * 2 + 1], y0, y1);
-        w[i] = pack2<T>(y0, y1);
       }
       __syncwarp();
       tmemStore32(colS + 32 * side, w);
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmemStoreWait();
       if (!whole) {
         // Values of keys that no row sees may be NaN, and 0 x NaN is NaN: the tile that uses the block first zeroes them, row r key r.
@@ -509,6 +556,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
       ++done;
     }
     // ---------------------------------------------------------------- output
+    pairBarrier(bar);                                 // both have read the last maximum
     storeShared(mineAt, l);
     if (ok && !mbarWait(&oFull[t], 0, abortWord)) { ok = false; atomicExch(&g_pagedChunkStatus, 12); }
     tcFenceAfter();

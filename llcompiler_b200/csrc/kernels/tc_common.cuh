@@ -146,6 +146,8 @@ __device__ __forceinline__ void fma2(float& x0, float& x1, float s0, float s1, f
 __device__ __forceinline__ void add2(float& x0, float& x1, float y0, float y1) {
   asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+f"(x0), "+f"(x1) : "f"(y0), "f"(y1));
 }
+// (p0, p1) = (p0, p1) * (r0, r1) + (c, c).
+__device__ __forceinline__ void horner2(float& p0, float& p1, float r0, float r1, float c) { fma2(p0, p1, r0, r1, c, c); }
 // geluTanhBf16 (common.cuh) of two values, the same operations on packed pairs.
 __device__ __forceinline__ void geluTanhBf16x2(float& x0, float& x1) {
   float u0, u1, h0, h1;
@@ -307,6 +309,13 @@ __device__ __forceinline__ void tmemStore32(uint32_t taddr, const uint32_t* r) {
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
         "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
         "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmemStore16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
