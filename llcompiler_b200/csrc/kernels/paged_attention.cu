@@ -128,7 +128,7 @@ int checkAndFill(const LlcPagedAttentionParams* p, PagedArgs* a) {
 // What the tensor-core kernels take: the types, head sizes and pages they have tiles for, and 16-byte steps everywhere.
 bool tensorTypes(const PagedArgs& a) {
   bool ok = a.dtype != LLC_FLOAT32 && (a.d == 64 || a.d == 128) && a.pageSize >= 16 && (a.pageSize & (a.pageSize - 1)) == 0 && a.numPages > 0 && a.reach > 0 &&
-            (long long)a.batch * a.kvHeads <= 0x7FFFFFFFLL;
+            (long long)a.batch * a.kvHeads <= 0x7FFFFFFFLL && a.tokens * a.group < 0x7FFFFF00LL;
   for (long long s : {a.qSt, a.qSh, a.oSt, a.oSh}) ok = ok && s % 8 == 0;
   for (long long s : {a.kcSp, a.kcSn, a.kcSh, a.vcSp, a.vcSn, a.vcSh}) ok = ok && s % 8 == 0 && s > 0 && s < (1LL << 38);
   for (const void* x : {a.q, a.k, a.v, (const void*)a.out}) ok = ok && (reinterpret_cast<uintptr_t>(x) & 15) == 0;

@@ -54,12 +54,12 @@ struct Tile {
   int first, last;             // places of its first and last token
   Seen seen;
 };
-__device__ __forceinline__ Tile tileOf(const PagedArgs& p, const Sequence& s, long long row0, long long rows) {
+__device__ __forceinline__ Tile tileOf(const PagedArgs& p, const Sequence& s, int row0, int rows) {
   Tile t;
-  const long long rowEnd = row0 + kTileRows < rows ? row0 + kTileRows : rows;
+  const int rowEnd = rows - row0 > kTileRows ? row0 + kTileRows : rows;
   if (row0 >= rowEnd) { t.first = 0; t.last = -1; t.seen = Seen{0, 0, 0}; return t; }
-  t.first = clipPlace((long long)s.len - s.n + row0 / p.group);
-  t.last = clipPlace((long long)s.len - s.n + (rowEnd - 1) / p.group);
+  t.first = clipPlace((long long)s.len - s.n + (uint32_t)row0 / (uint32_t)p.group);
+  t.last = clipPlace((long long)s.len - s.n + (uint32_t)(rowEnd - 1) / (uint32_t)p.group);
   t.seen = seenBy(p, t.first, t.last);
   return t;
 }
@@ -98,7 +98,7 @@ struct Plan {
   int begin, end;              // units of this CTA's part of the keys
   int seq, tile;               // sequence (-1: nothing to do) and pair of tiles
   int n, len;                  // of the sequence
-  long long row0, rows, qBegin;
+  int row0, rows, qBegin;      // rows (token, query head) of the sequence: the host keeps tokens x query heads below 2^31
 };
 
 // Barriers by their shared-memory address (a generic pointer costs two registers and a conversion at every use).
@@ -125,8 +125,8 @@ __device__ __forceinline__ void commitAt(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-__device__ __forceinline__ long long tilesOf(const PagedArgs& p, int b, int doneRows) {
-  const long long rows = (long long)sequenceOf(p, b).n * p.group;
+__device__ __forceinline__ int tilesOf(const PagedArgs& p, const Sequence& s, int doneRows) {
+  const int rows = s.n * p.group;
   return rows <= doneRows ? 0 : (rows + kCtaRows - 1) / kCtaRows;
 }
 
@@ -216,7 +216,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
   uint64_t* qReady = oFull + 2;                       // both tiles of Q written
   uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(misc + 256);
   volatile int* abortWord = reinterpret_cast<volatile int*>(misc + 260);
-  long long* sScan = reinterpret_cast<long long*>(misc + 264);   // [20]
+  int* sScan = reinterpret_cast<int*>(misc + 272);               // [20]
   Plan* plan = reinterpret_cast<Plan*>(misc + 512);
   float* sRow = reinterpret_cast<float*>(misc + 1024);           // [2 tiles][2 halves][128]
   const PagedArgs& p = a.p;
@@ -233,12 +233,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
   // most keys of its sequence.
   const int h = blockIdx.x / a.splits, split = blockIdx.x - h * a.splits;
   {
+    // a thread keeps its (last) sequence: with up to kThreads of them nothing is read twice
     const int per = (p.batch + kThreads - 1) / kThreads, first = threadIdx.x * per;
-    long long mine = 0;
-    for (int i = first; i < first + per && i < p.batch; ++i) mine += tilesOf(p, i, a.doneRows);
-    long long run = mine;
+    int mine = 0;
+    Sequence s{};
+    for (int i = first; i < first + per && i < p.batch; ++i) { s = sequenceOf(p, i); mine += tilesOf(p, s, a.doneRows); }
+    int run = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += x; }
+    for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += x; }
     if (lane == 31) sScan[warp] = run;
     if (threadIdx.x == 0) {
       plan->seq = -1;
@@ -249,18 +251,21 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
       fenceBarrierInit();
     }
     __syncthreads();
-    long long before = run - mine, all = 0;
-    for (int w = 0; w < kThreads / 32; ++w) { if (w < warp) before += sScan[w]; all += sScan[w]; }
-    const long long want = all - 1 - (long long)blockIdx.y;
+    int before = run - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) { const int x = sScan[w]; if (w < warp) before += x; all += x; }
+    const int want = all - 1 - (int)blockIdx.y;
     if (want >= before && want < before + mine) {
       int i = first;
-      for (; i < first + per; ++i) {
-        const long long c = tilesOf(p, i, a.doneRows);
-        if (want < before + c) break;
-        before += c;
+      if (per > 1) {
+        for (; i < first + per; ++i) {
+          s = sequenceOf(p, i);
+          const int c = tilesOf(p, s, a.doneRows);
+          if (want < before + c) break;
+          before += c;
+        }
       }
-      const Sequence s = sequenceOf(p, i);
-      const long long rows = (long long)s.n * p.group, row0 = (want - before) * kCtaRows;
+      const int rows = s.n * p.group, row0 = (want - before) * kCtaRows;
       const Tile tile0 = tileOf(p, s, row0, rows), tile1 = tileOf(p, s, row0 + kTileRows, rows);
       plan->seen = seenBy(p, tile0.first, tile1.last >= 0 ? tile1.last : tile0.last);
       const Blocks bl = blocksOf(plan->seen, kKeys);
@@ -270,15 +275,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
       plan->bl = bl;
       plan->begin = begin;
       plan->end = begin + share < bl.count ? begin + share : bl.count;
-      plan->seq = i; plan->tile = (int)(want - before); plan->n = s.n; plan->len = s.len;
-      plan->row0 = row0; plan->rows = rows; plan->qBegin = s.begin;
+      plan->seq = i; plan->tile = want - before; plan->n = s.n; plan->len = s.len;
+      plan->row0 = row0; plan->rows = rows; plan->qBegin = (int)s.begin;
     }
     __syncthreads();
   }
   const long long pair = (long long)blockIdx.y * p.kvHeads + h;
   if (a.splits > 1 && split == 0 && threadIdx.x == 0) a.records[pair] = make_int4(plan->seq, plan->tile, 0, 0);
   if (plan->seq < 0) return;                          // fewer tiles than the grid has room for
-
   if (warp == kIssuerWarp) tmemAlloc(tmemSlot, 512);
   tcFenceBefore();
   __syncthreads();
@@ -410,30 +414,38 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     const int t = warp >> 3, side = (warp >> 2) & 1, q4 = warp & 3, r = q4 * 32 + lane;   // tile, half of the columns, row
     // this thread's row: its place, and where it lies in q and out (worked out again after the loop)
     auto liveRow = [&]() { return plan->row0 + t * kTileRows + r < plan->rows; };
-    auto offsetOf = [&](long long sTok, long long sHead) {
-      const long long row = plan->row0 + t * kTileRows + r, x = row < plan->rows ? row : plan->rows - 1, tok = x / p.group;
-      return (plan->qBegin + tok) * sTok + (h * p.group + (x - tok * p.group)) * sHead;
+    auto tokenOf = [&](int& head) {
+      const uint32_t row = plan->row0 + t * kTileRows + r, x = min(row, (uint32_t)plan->rows - 1u), tok = x / (uint32_t)p.group;
+      head = h * p.group + (int)(x - tok * p.group);
+      return (int)tok;
     };
-    const long long row = plan->row0 + t * kTileRows + r;
-    const int pos = clipPlace((long long)plan->len - plan->n + (row < plan->rows ? row : plan->rows - 1) / p.group);
+    int head;
+    const int tok = tokenOf(head), pos = clipPlace((long long)plan->len - plan->n + tok);
     uint8_t* tileQ = sQ + t * C::kTile;
     const uint32_t mineAt = smemAddr(sRow + (t * 2 + side) * kTileRows + r), otherAt = smemAddr(sRow + (t * 2 + (side ^ 1)) * kTileRows + r);
     const int bar = 1 + t * 4 + q4;                   // the two warps that share 32 rows
     constexpr int kChunks = D / 8;                    // 16-byte chunks of a row
     constexpr int kRowsAtOnce = 32 / kChunks;         // rows that a warp's 16-byte accesses cover
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-    const long long qOff = offsetOf(p.qSt, p.qSh);
+    const long long qOff = (long long)(plan->qBegin + tok) * p.qSt + head * p.qSh;
     const bool inQ = liveRow();
+    {
     // Q, a warp 16 of its 32 rows: neighbouring lanes take neighbouring chunks of a row
-#pragma unroll 4
-    for (int i = 0; i < 16; i += kRowsAtOnce) {
-      const int src = side * 16 + i + lane / kChunks, c = lane % kChunks, rr = q4 * 32 + src;
+    uint4 x[16 / kRowsAtOnce];
+#pragma unroll
+    for (int i = 0; i < 16 / kRowsAtOnce; ++i) {
+      const int src = side * 16 + i * kRowsAtOnce + lane / kChunks;
       const long long off = __shfl_sync(0xffffffffu, qOff, src);
       const bool in = __shfl_sync(0xffffffffu, (int)inQ, src);
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (in) x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + off + c * 8);
-      if (a.signQ < 0.f) { x.x ^= 0x80008000u; x.y ^= 0x80008000u; x.z ^= 0x80008000u; x.w ^= 0x80008000u; }
-      *reinterpret_cast<uint4*>(tileQ + (c >> 3) * C::kAtom + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (in) x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + off + lane % kChunks * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / kRowsAtOnce; ++i) {
+      const int c = lane % kChunks, rr = q4 * 32 + side * 16 + i * kRowsAtOnce + lane / kChunks;
+      if (a.signQ < 0.f) { x[i].x ^= 0x80008000u; x[i].y ^= 0x80008000u; x[i].z ^= 0x80008000u; x[i].w ^= 0x80008000u; }
+      *reinterpret_cast<uint4*>(tileQ + (c >> 3) * C::kAtom + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x[i];
+    }
     }
     fenceProxyAsync();
     __syncwarp();
@@ -580,8 +592,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = 0.f;
       }
+      float zero = 0.f;                               // stays 0 unless some element is NaN or infinite
 #pragma unroll
-      for (int i = 0; i < 32; ++i) odd = odd || !(fabsf(o[i]) <= 3.402823466e38f);
+      for (int i = 0; i < 32; ++i) zero = fmaf(o[i], 0.f, zero);
+      odd = odd || zero != 0.f;
       const int col = side * (D / 2) + c;
       if (cut) {
 #pragma unroll
@@ -599,13 +613,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     }
     pairBarrier(bar);
     const bool live = liveRow();
-    const long long qAt = offsetOf(p.qSt, p.qSh), oOff = offsetOf(p.oSt, p.oSh);
+    int oHead;
+    const int oTok = tokenOf(oHead);
     unsigned redo = __ballot_sync(0xffffffffu, odd && live && fabsf(l) <= 3.402823466e38f);
     while (redo) {
       const int src = __ffs(redo) - 1, rr = q4 * 32 + src;
       redo &= redo - 1;
       float o[D / 32];
-      sumRow<T, D>(a, plan->seq, h, __shfl_sync(0xffffffffu, qAt, src), __shfl_sync(0xffffffffu, pos, src), plan->bl, plan->begin, plan->end, __shfl_sync(0xffffffffu, base, src), o);
+      sumRow<T, D>(a, plan->seq, h, __shfl_sync(0xffffffffu, (long long)(plan->qBegin + oTok) * p.qSt + oHead * p.qSh, src), __shfl_sync(0xffffffffu, pos, src), plan->bl, plan->begin, plan->end, __shfl_sync(0xffffffffu, base, src), o);
       const float f = __shfl_sync(0xffffffffu, inv, src);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
@@ -620,6 +635,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     }
     pairBarrier(bar);
     if (!cut) {
+      const long long oOff = (long long)(plan->qBegin + oTok) * p.oSt + oHead * p.oSh;
 #pragma unroll 4
       for (int i = 0; i < 16; i += kRowsAtOnce) {
         const int src = side * 16 + i + lane / kChunks, c = lane % kChunks, rr = q4 * 32 + src;
