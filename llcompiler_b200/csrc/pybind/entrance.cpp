@@ -7,7 +7,7 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
-#include <array>
+#include <cmath>
 #include <cstring>
 #include <stdexcept>
 #include <string>
@@ -164,58 +164,237 @@ struct Execution {
   int64_t arena_bytes() const { need(); return llc_arena_bytes(exec); }
 };
 
-// Operators of the kernel library that a serving loop calls on device tensors directly, without a compiled plan: addresses,
-// extents and strides in, one launch on `stream` out.  The Python side (executor/paged.py) looks after shapes and devices.
-template <size_t N> using Ints = std::array<int64_t, N>;
-const void* at(int64_t p) { return reinterpret_cast<const void*>(static_cast<uintptr_t>(p)); }
-void* to(int64_t p) { return reinterpret_cast<void*>(static_cast<uintptr_t>(p)); }
+// ---- Operators of the kernel library that a serving loop calls on device tensors directly, without a compiled plan
+// (llcompiler_b200/executor/paged.py).  A decoding step makes a handful of such calls of a few microseconds each, so the checks are
+// made here: what a tensor says of itself is read through the interpreter once, nothing links against the tensor library.
+struct Torch {
+  py::object tensor, emptyLike, empty, stream, gradEnabled;
+  py::object f32, f16, bf16, f64, i32, i64;
+  PyObject* nShape, *nStride, *nDtype, *nPtr, *nDevice, *nGrad;
+  Torch() {
+    py::module_ t = py::module_::import("torch"), c = py::module_::import("torch._C");
+    tensor = t.attr("Tensor"); emptyLike = t.attr("empty_like"); empty = t.attr("empty"); gradEnabled = t.attr("is_grad_enabled");
+    stream = c.attr("_cuda_getCurrentRawStream");
+    f32 = t.attr("float32"); f16 = t.attr("float16"); bf16 = t.attr("bfloat16"); f64 = t.attr("float64"); i32 = t.attr("int32"); i64 = t.attr("int64");
+    nShape = PyUnicode_InternFromString("shape"); nStride = PyUnicode_InternFromString("stride"); nDtype = PyUnicode_InternFromString("dtype");
+    nPtr = PyUnicode_InternFromString("data_ptr"); nDevice = PyUnicode_InternFromString("get_device"); nGrad = PyUnicode_InternFromString("requires_grad");
+  }
+  int code(PyObject* d) const {
+    if (d == bf16.ptr()) return LLC_BFLOAT16;
+    if (d == f16.ptr()) return LLC_FLOAT16;
+    if (d == f32.ptr()) return LLC_FLOAT32;
+    if (d == i32.ptr()) return LLC_INT32;
+    if (d == i64.ptr()) return LLC_INT64;
+    if (d == f64.ptr()) return LLC_FLOAT64;
+    return -1;
+  }
+};
+const Torch& torch() { static Torch* t = new Torch(); return *t; }   // never destroyed: the interpreter may be gone by then
 
-// pointers: x, out, positions, inv_freq; sizes: tokens, heads, d, pairs; strides: x_st, x_sh, o_st, o_sh, pos_sa
-void rotary(const Ints<4>& ptr, int dtype, int pos_dtype, const Ints<4>& n, const Ints<5>& s, int axes, const Ints<4>& sections, bool interleaved, uintptr_t stream) {
+py::object got(PyObject* o) { if (!o) throw py::error_already_set(); return py::reinterpret_steal<py::object>(o); }
+
+// One operand.  `name` goes into the message when something does not fit.
+struct Operand {
+  const char* name;
+  int rank = 0, dtype = -1, device = -1;
+  int64_t n[4] = {1, 1, 1, 1}, s[4] = {0, 0, 0, 0};
+  uintptr_t ptr = 0;
+  [[noreturn]] void bad(const std::string& what) const { throw py::value_error(std::string(name) + ": " + what); }
+  std::string shape() const {
+    std::string r = "(";
+    for (int i = 0; i < rank; ++i) r += (i ? ", " : "") + std::to_string(n[i]);
+    return r + ")";
+  }
+  Operand(const char* name_, py::handle h, int least, int most) : name(name_) {
+    const Torch& t = torch();
+    PyObject* o = h.ptr();
+    if (!PyObject_TypeCheck(o, reinterpret_cast<PyTypeObject*>(t.tensor.ptr()))) throw py::type_error(std::string(name) + ": expected a tensor, got " + Py_TYPE(o)->tp_name);
+    py::object sh = got(PyObject_GetAttr(o, t.nShape)), st = got(PyObject_CallMethodNoArgs(o, t.nStride)), dt = got(PyObject_GetAttr(o, t.nDtype)),
+               dv = got(PyObject_CallMethodNoArgs(o, t.nDevice)), gr = got(PyObject_GetAttr(o, t.nGrad)), pt = got(PyObject_CallMethodNoArgs(o, t.nPtr));
+    rank = (int)PyTuple_GET_SIZE(sh.ptr());
+    if (rank < least || rank > most) throw py::value_error(std::string(name) + ": expected " + std::to_string(least) + " dims, got " + std::to_string(rank));
+    for (int i = 0; i < rank; ++i) { n[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(sh.ptr(), i)); s[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(st.ptr(), i)); }
+    dtype = t.code(dt.ptr());
+    device = (int)PyLong_AsLong(dv.ptr());
+    ptr = (uintptr_t)PyLong_AsUnsignedLongLong(pt.ptr());
+    if (PyErr_Occurred()) throw py::error_already_set();
+    if (device < 0) bad("expected a CUDA tensor; there is no CPU fallback");
+    if (gr.ptr() == Py_True && t.gradEnabled().cast<bool>()) bad("inference only, it requires a gradient");
+  }
+  void on(int dev) const { if (device != dev) bad("on cuda:" + std::to_string(device) + ", expected cuda:" + std::to_string(dev)); }
+  void type(int want, const char* said) const { if (dtype != want) bad(std::string("expected ") + said); }
+  void unit(int dim, const char* what) const { if (n[dim] > 1 && s[dim] != 1) bad(std::string(what) + " must have unit stride"); }
+};
+// [tokens, heads, head_dim]
+Operand rows(const char* name, py::handle h) { Operand o(name, h, 3, 3); o.unit(2, "the head dim"); return o; }
+Operand rowsLike(const char* name, py::handle h, const Operand& first) {
+  Operand o = rows(name, h);
+  o.on(first.device);
+  if (o.dtype != first.dtype) o.bad(std::string("expected the type of ") + first.name);
+  return o;
+}
+Operand firstRows(const char* name, py::handle h) {
+  Operand o = rows(name, h);
+  if (o.dtype != LLC_FLOAT32 && o.dtype != LLC_BFLOAT16 && o.dtype != LLC_FLOAT16) o.bad("expected float32, bfloat16 or float16");
+  return o;
+}
+// The result's tensor: the caller's, or a new one.
+Operand output(const char* name, py::object& out, py::handle like, const Operand& l) {
+  const bool own = out.is_none();
+  if (own) {
+    out = torch().emptyLike(like);
+    Operand o(name, out, 3, 3);
+    if (l.n[2] <= 1 || o.s[2] == 1) return o;
+    out = torch().empty(like.attr("shape"), py::arg("dtype") = like.attr("dtype"), py::arg("device") = like.attr("device"));
+  }
+  Operand o = rowsLike(name, out, l);
+  for (int i = 0; i < 3; ++i) {
+    if (o.n[i] != l.n[i]) o.bad("expected shape " + l.shape() + ", got " + o.shape());
+    if (o.n[i] > 1 && o.s[i] == 0) o.bad("an output may not repeat its elements (stride 0)");
+  }
+  return o;
+}
+
+struct Turns { uintptr_t positions = 0, freq = 0; int posType = LLC_INT64, axes = 0; int64_t posStride = 0, pairs = 0; int32_t sections[LLC_ROTARY_MAX_AXES] = {0, 0, 0, 0}; };
+Turns turns(py::handle positions, py::handle freq, py::handle sections, int64_t tokens, int64_t d, int device) {
+  Turns t;
+  Operand f("inv_freq", freq, 1, 1);
+  f.on(device);
+  f.type(LLC_FLOAT64, "float64");
+  f.unit(0, "it");
+  t.freq = f.ptr;
+  t.pairs = f.n[0];
+  if (t.pairs < 1 || 2 * t.pairs > d) f.bad(std::to_string(t.pairs) + " pairs do not fit a head of " + std::to_string(d));
+  if (sections.is_none()) {
+    t.axes = 1;
+    t.sections[0] = (int32_t)t.pairs;
+  } else {
+    py::object list = got(PySequence_Fast(sections.ptr(), "sections: expected a sequence of numbers"));
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(list.ptr());
+    int64_t sum = 0;
+    bool fits = n >= 1 && n <= LLC_ROTARY_MAX_AXES;
+    for (Py_ssize_t i = 0; fits && i < n; ++i) {
+      const long long x = PyLong_AsLongLong(PySequence_Fast_GET_ITEM(list.ptr(), i));
+      if (x == -1 && PyErr_Occurred()) throw py::error_already_set();
+      fits = x >= 0 && x <= t.pairs;
+      if (fits) { t.sections[i] = (int32_t)x; sum += x; }
+    }
+    if (!fits || sum != t.pairs) throw py::value_error("sections: expected 1 to 4 numbers that add up to " + std::to_string(t.pairs) + " pairs");
+    t.axes = (int)n;
+  }
+  if (positions.is_none()) return t;
+  Operand p("positions", positions, 1, 2);
+  p.on(device);
+  if (p.dtype != LLC_INT32 && p.dtype != LLC_INT64) p.bad("expected int32 or int64");
+  const int last = p.rank - 1;
+  if (p.n[last] != tokens || (last ? p.n[0] : 1) != t.axes) p.bad("expected shape (" + std::to_string(t.axes) + ", " + std::to_string(tokens) + "), got " + p.shape());
+  p.unit(last, "the tokens");
+  t.positions = p.ptr; t.posType = p.dtype; t.posStride = last ? p.s[0] : 0;
+  return t;
+}
+
+struct Batch { int64_t size, width, stride; const int32_t *table, *start, *len; int32_t* bad; };
+Batch batchOf(py::handle table, py::handle start, py::handle len, py::handle bad, int device) {
+  Operand t("page_table", table, 2, 2), s("q_start", start, 1, 1), l("kv_len", len, 1, 1);
+  for (const Operand* o : {&t, &s, &l}) { o->on(device); o->type(LLC_INT32, "int32"); o->unit(o->rank - 1, "the last dim"); }
+  if (s.n[0] != t.n[0] + 1) s.bad("expected " + std::to_string(t.n[0] + 1) + " entries, got " + std::to_string(s.n[0]));
+  if (l.n[0] != t.n[0]) l.bad("expected " + std::to_string(t.n[0]) + " entries, got " + std::to_string(l.n[0]));
+  Batch b{t.n[0], t.n[1], t.s[0], reinterpret_cast<const int32_t*>(t.ptr), reinterpret_cast<const int32_t*>(s.ptr), reinterpret_cast<const int32_t*>(l.ptr), nullptr};
+  if (!bad.is_none()) {
+    Operand x("bad_pages", bad, 1, 1);
+    x.on(device);
+    x.type(LLC_INT32, "int32");
+    if (x.n[0] != 1) x.bad("expected one counter");
+    b.bad = reinterpret_cast<int32_t*>(x.ptr);
+  }
+  return b;
+}
+Operand cacheOf(const char* name, py::handle h, const Operand& first) {
+  Operand c(name, h, 4, 4);
+  c.on(first.device);
+  if (c.dtype != first.dtype) c.bad(std::string("expected the type of ") + first.name);
+  c.unit(3, "the head dim");
+  if (c.n[1] < 1 || c.n[2] < 1) c.bad("empty pages, shape " + c.shape());
+  return c;
+}
+void sameShape(const Operand& a, const Operand& b) {
+  for (int i = 0; i < a.rank; ++i) if (a.n[i] != b.n[i]) b.bad("expected shape " + a.shape() + ", got " + b.shape());
+}
+void* streamOf(int device) { return reinterpret_cast<void*>(torch().stream(device).cast<uintptr_t>()); }
+template <typename T = void> T* at(uintptr_t p) { return reinterpret_cast<T*>(p); }
+
+py::object rotary(py::handle x, py::handle positions, py::handle freq, py::handle sections, bool interleaved, py::object out) {
+  Operand a = firstRows("x", x);
+  if (positions.is_none()) throw py::value_error("positions: required");
+  const Turns t = turns(positions, freq, sections, a.n[0], a.n[2], a.device);
+  const Operand o = output("out", out, x, a);
   LlcRotaryParams p{};
-  p.x = at(ptr[0]); p.out = to(ptr[1]); p.positions = at(ptr[2]); p.inv_freq = static_cast<const double*>(at(ptr[3]));
-  p.dtype = dtype; p.pos_dtype = pos_dtype; p.tokens = n[0]; p.heads = n[1]; p.d = n[2]; p.pairs = n[3];
-  p.x_st = s[0]; p.x_sh = s[1]; p.o_st = s[2]; p.o_sh = s[3]; p.pos_sa = s[4]; p.axes = axes; p.interleaved = interleaved;
-  for (int i = 0; i < 4; ++i) p.sections[i] = (int32_t)sections[i];
-  check(llc_cuda_rotary(&p, reinterpret_cast<void*>(stream)));
+  p.x = at(a.ptr); p.out = at(o.ptr); p.positions = at(t.positions); p.inv_freq = at<const double>(t.freq);
+  p.dtype = a.dtype; p.pos_dtype = t.posType; p.tokens = a.n[0]; p.heads = a.n[1]; p.d = a.n[2]; p.pairs = t.pairs;
+  p.x_st = a.s[0]; p.x_sh = a.s[1]; p.o_st = o.s[0]; p.o_sh = o.s[1]; p.pos_sa = t.posStride; p.axes = t.axes; p.interleaved = interleaved;
+  std::memcpy(p.sections, t.sections, sizeof p.sections);
+  check(llc_cuda_rotary(&p, streamOf(a.device)));
+  return out;
 }
 
-// pointers: k, v, k_cache, v_cache, q, q_out, page_table, q_start, kv_len, positions, inv_freq, bad_pages; sizes: tokens, batch, heads, kv_heads, d,
-// pairs, num_pages, page_size, table_width, table_s0; strides: q_st, q_sh, qo_st, qo_sh, k_st, k_sh, v_st, v_sh, then page, slot and head of each cache, pos_sa
-void kvAppend(const Ints<12>& ptr, int dtype, int pos_dtype, const Ints<10>& n, const Ints<15>& s, int axes, const Ints<4>& sections, bool interleaved, uintptr_t stream) {
+py::object kvAppend(py::handle k, py::handle v, py::handle kCache, py::handle vCache, py::handle table, py::handle start, py::handle len, py::handle q, py::handle positions,
+                    py::handle freq, py::handle sections, bool interleaved, py::object qOut, py::handle bad) {
+  Operand a = firstRows("k", k), b = rowsLike("v", v, a), kc = cacheOf("k_cache", kCache, a), vc = cacheOf("v_cache", vCache, a);
+  sameShape(a, b);
+  sameShape(kc, vc);
+  if (a.n[1] != kc.n[2] || a.n[2] != kc.n[3]) a.bad("expected [tokens, " + std::to_string(kc.n[2]) + ", " + std::to_string(kc.n[3]) + "], got " + a.shape());
+  const Batch s = batchOf(table, start, len, bad, a.device);
   LlcKvAppendParams p{};
-  p.k = at(ptr[0]); p.v = at(ptr[1]); p.k_cache = to(ptr[2]); p.v_cache = to(ptr[3]); p.q = at(ptr[4]); p.q_out = to(ptr[5]);
-  p.page_table = static_cast<const int32_t*>(at(ptr[6])); p.q_start = static_cast<const int32_t*>(at(ptr[7])); p.kv_len = static_cast<const int32_t*>(at(ptr[8]));
-  p.positions = at(ptr[9]); p.inv_freq = static_cast<const double*>(at(ptr[10])); p.bad_pages = static_cast<int32_t*>(to(ptr[11]));
-  p.dtype = dtype; p.pos_dtype = pos_dtype;
-  p.tokens = n[0]; p.batch = n[1]; p.heads = n[2]; p.kv_heads = n[3]; p.d = n[4]; p.pairs = n[5]; p.num_pages = n[6]; p.page_size = n[7]; p.table_width = n[8]; p.table_s0 = n[9];
-  p.q_st = s[0]; p.q_sh = s[1]; p.qo_st = s[2]; p.qo_sh = s[3]; p.k_st = s[4]; p.k_sh = s[5]; p.v_st = s[6]; p.v_sh = s[7];
-  p.kc_sp = s[8]; p.kc_sn = s[9]; p.kc_sh = s[10]; p.vc_sp = s[11]; p.vc_sn = s[12]; p.vc_sh = s[13]; p.pos_sa = s[14];
-  p.axes = axes; p.interleaved = interleaved;
-  for (int i = 0; i < 4; ++i) p.sections[i] = (int32_t)sections[i];
-  check(llc_cuda_kv_append(&p, reinterpret_cast<void*>(stream)));
+  if (!q.is_none()) {
+    Operand x = rowsLike("q", q, a);
+    if (x.n[0] != a.n[0] || x.n[2] != a.n[2]) x.bad("expected [" + std::to_string(a.n[0]) + ", heads, " + std::to_string(a.n[2]) + "], got " + x.shape());
+    const Operand o = output("q_out", qOut, q, x);
+    p.q = at(x.ptr); p.q_out = at(o.ptr); p.heads = x.n[1]; p.q_st = x.s[0]; p.q_sh = x.s[1]; p.qo_st = o.s[0]; p.qo_sh = o.s[1];
+  } else if (!qOut.is_none()) {
+    throw py::value_error("q_out: no queries were given");
+  }
+  if (!freq.is_none()) {
+    const Turns t = turns(positions, freq, sections, a.n[0], a.n[2], a.device);
+    p.positions = at(t.positions); p.inv_freq = at<const double>(t.freq); p.pos_dtype = t.posType; p.pairs = t.pairs; p.pos_sa = t.posStride; p.axes = t.axes;
+    std::memcpy(p.sections, t.sections, sizeof p.sections);
+  } else if (!positions.is_none() || !sections.is_none()) {
+    throw py::value_error("positions and sections: no inv_freq was given");
+  }
+  p.k = at(a.ptr); p.v = at(b.ptr); p.k_cache = at(kc.ptr); p.v_cache = at(vc.ptr); p.page_table = s.table; p.q_start = s.start; p.kv_len = s.len; p.bad_pages = s.bad;
+  p.dtype = a.dtype; p.tokens = a.n[0]; p.batch = s.size; p.kv_heads = a.n[1]; p.d = a.n[2]; p.num_pages = kc.n[0]; p.page_size = kc.n[1]; p.table_width = s.width;
+  p.table_s0 = s.stride; p.k_st = a.s[0]; p.k_sh = a.s[1]; p.v_st = b.s[0]; p.v_sh = b.s[1];
+  p.kc_sp = kc.s[0]; p.kc_sn = kc.s[1]; p.kc_sh = kc.s[2]; p.vc_sp = vc.s[0]; p.vc_sn = vc.s[1]; p.vc_sh = vc.s[2]; p.interleaved = interleaved;
+  check(llc_cuda_kv_append(&p, streamOf(a.device)));
+  return qOut;
 }
 
-// pointers: q, k_cache, v_cache, out, page_table, q_start, kv_len, bad_pages; sizes: tokens, batch, heads, kv_heads, d, max_q, num_pages, page_size, table_width,
-// table_s0, window, sinks; strides: q_st, q_sh, o_st, o_sh, then page, slot and head of each cache
-LlcPagedAttentionParams pagedParams(const Ints<8>& ptr, int dtype, float scale, const Ints<12>& n, const Ints<10>& s) {
+py::object pagedAttention(py::handle q, py::handle kCache, py::handle vCache, py::handle table, py::handle start, py::handle len, py::object scale, int64_t window, int64_t sinks,
+                          py::object maxQ, py::object out, py::handle bad) {
+  Operand a = firstRows("q", q), kc = cacheOf("k_cache", kCache, a), vc = cacheOf("v_cache", vCache, a);
+  sameShape(kc, vc);
+  const int64_t kv = kc.n[2], d = kc.n[3];
+  if (a.n[2] != d || a.n[1] == 0 || a.n[1] % kv) a.bad("expected [tokens, a multiple of " + std::to_string(kv) + ", " + std::to_string(d) + "], got " + a.shape());
+  const Batch s = batchOf(table, start, len, bad, a.device);
+  if (window < 0 || sinks < 0) throw py::value_error("window and sinks: must not be negative");
+  const int64_t most = maxQ.is_none() ? a.n[0] : maxQ.cast<int64_t>();
+  if (most < 0) throw py::value_error("max_q: must not be negative");
+  const Operand o = output("out", out, q, a);
   LlcPagedAttentionParams p{};
-  p.q = at(ptr[0]); p.k_cache = at(ptr[1]); p.v_cache = at(ptr[2]); p.out = to(ptr[3]);
-  p.page_table = static_cast<const int32_t*>(at(ptr[4])); p.q_start = static_cast<const int32_t*>(at(ptr[5])); p.kv_len = static_cast<const int32_t*>(at(ptr[6]));
-  p.bad_pages = static_cast<int32_t*>(to(ptr[7])); p.dtype = dtype; p.scale = scale;
-  p.tokens = n[0]; p.batch = n[1]; p.heads = n[2]; p.kv_heads = n[3]; p.d = n[4]; p.max_q = n[5]; p.num_pages = n[6]; p.page_size = n[7]; p.table_width = n[8];
-  p.table_s0 = n[9]; p.window = n[10]; p.sinks = n[11];
-  p.q_st = s[0]; p.q_sh = s[1]; p.o_st = s[2]; p.o_sh = s[3]; p.kc_sp = s[4]; p.kc_sn = s[5]; p.kc_sh = s[6]; p.vc_sp = s[7]; p.vc_sn = s[8]; p.vc_sh = s[9];
-  return p;
-}
-int64_t pagedWorkspace(const Ints<8>& ptr, int dtype, float scale, const Ints<12>& n, const Ints<10>& s) {
-  LlcPagedAttentionParams p = pagedParams(ptr, dtype, scale, n, s);
-  return llc_cuda_paged_attention_workspace(&p);
-}
-void pagedAttention(const Ints<8>& ptr, int dtype, float scale, const Ints<12>& n, const Ints<10>& s, uintptr_t workspace, int64_t bytes, uintptr_t stream) {
-  LlcPagedAttentionParams p = pagedParams(ptr, dtype, scale, n, s);
-  p.workspace = reinterpret_cast<void*>(workspace); p.workspace_bytes = bytes;
-  check(llc_cuda_paged_attention(&p, reinterpret_cast<void*>(stream)));
+  p.q = at(a.ptr); p.k_cache = at(kc.ptr); p.v_cache = at(vc.ptr); p.out = at(o.ptr); p.page_table = s.table; p.q_start = s.start; p.kv_len = s.len; p.bad_pages = s.bad;
+  p.dtype = a.dtype; p.scale = scale.is_none() ? (float)(1.0 / std::sqrt((double)d)) : scale.cast<float>();
+  p.tokens = a.n[0]; p.batch = s.size; p.heads = a.n[1]; p.kv_heads = kv; p.d = d; p.max_q = most; p.num_pages = kc.n[0]; p.page_size = kc.n[1];
+  p.table_width = s.width; p.table_s0 = s.stride; p.window = window; p.sinks = sinks;
+  p.q_st = a.s[0]; p.q_sh = a.s[1]; p.o_st = o.s[0]; p.o_sh = o.s[1];
+  p.kc_sp = kc.s[0]; p.kc_sn = kc.s[1]; p.kc_sh = kc.s[2]; p.vc_sp = vc.s[0]; p.vc_sn = vc.s[1]; p.vc_sh = vc.s[2];
+  // scratch from the caching allocator at every call: ordered with the stream, and a captured graph gets memory of its own
+  py::object scratch;
+  if (const int64_t bytes = llc_cuda_paged_attention_workspace(&p)) {
+    scratch = torch().empty((bytes + 3) / 4, py::arg("dtype") = torch().f32, py::arg("device") = q.attr("device"));
+    p.workspace = at(scratch.attr("data_ptr")().cast<uintptr_t>());
+    p.workspace_bytes = bytes;
+  }
+  check(llc_cuda_paged_attention(&p, streamOf(a.device)));
+  return out;
 }
 
 }  // namespace
@@ -272,7 +451,6 @@ PYBIND11_MODULE(llcompiler_, m) {
   auto ops = m.def_submodule("ops");
   ops.def("rotary", &rotary);
   ops.def("kv_append", &kvAppend);
-  ops.def("paged_attention_workspace", &pagedWorkspace);
   ops.def("paged_attention", &pagedAttention);
   m.def("version", []() { return std::string(llc_version()); });
 }
