@@ -7,9 +7,10 @@ __all__ = ["ExecutionEngine", "Torch_ExecutionEngine", "BatchShardedRunner", "ga
 def __getattr__(name):
     # the engines and the decoder operators need the llcompiler_ extension (and a GPU); the sharding helpers do not
     if name in ("ExecutionEngine", "Torch_ExecutionEngine", "TORCH_DTYPE_TO_TYPE"):
-        from . import engine
-        return getattr(engine, name)
-    if name in ("rotary", "kv_append", "paged_attention"):
-        from . import paged
-        return getattr(paged, name)
-    raise AttributeError(name)
+        from . import engine as module
+    elif name in ("rotary", "kv_append", "paged_attention"):
+        from . import paged as module
+    else:
+        raise AttributeError(name)
+    value = globals()[name] = getattr(module, name)      # found without this function from now on
+    return value
