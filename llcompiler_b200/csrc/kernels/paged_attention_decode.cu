@@ -25,6 +25,7 @@ using namespace tc;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 16;                          // keys of a block
+constexpr int kTail = 4;                           // floats behind a part's row of sums: its maximum, its sum of weights, two unused
 
 template <int D, int MT> struct Config {
   static constexpr int kRows = 16 * MT;
@@ -44,8 +45,9 @@ struct DecodeArgs {
   PagedArgs p;
   int pageShift, minBlocks;    // page_size = 1 << pageShift; least share of a warp
   int slotRows;                // rows of a slot: the most that a sequence of this call has
+  int joinRows;                // rows of a block of the joining kernel
   int2* records;               // [pairs]: first warp of the pair, number of warps that have a part of it
-  float* slots;                // [pairs + warps][slotRows][D + 2]: a part's sums, its maximum, its sum of weights; slot = pair + warp
+  float* slots;                // [pairs + warps][slotRows][D + kTail]: a part's sums; slot = pair + warp
 };
 
 // The blocks of keys of one key head of a sequence; one empty block where nothing is visible, which writes the zeros; none where the
@@ -381,7 +383,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
       const bool whole = begin == 0 && use.end == use.bl.count;
       const long long pair = (long long)use.b * p.kvHeads + use.h;
       if (begin == 0 && lane == 0) a.records[pair] = make_int2((int)me, 1 + (int)((use.bl.count - use.end + share - 1) / share));
-      float* slot = a.slots + (pair + me) * a.slotRows * (D + 2);
+      float* slot = a.slots + (pair + me) * a.slotRows * (D + kTail);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -395,7 +397,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
 #pragma unroll
             for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint32_t*>(dst + 8 * i) = pack2<T>(o[mt][i][2 * r] * inv, o[mt][i][2 * r + 1] * inv);
           } else {
-            float* dst = slot + row * (D + 2);
+            float* dst = slot + row * (D + kTail);
 #pragma unroll
             for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(dst + 8 * i + c4 * 2) = make_float2(o[mt][i][2 * r], o[mt][i][2 * r + 1]);
             if (c4 == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[mt][r], l[mt][r]);
@@ -460,50 +462,99 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
     for (int i = 0; i < 1000; ++i) __nanosleep(1000);   // copies in flight land before the CTA gives its memory back
 }
 
-// Joins the parts of a pair that was cut: block (pair, row).  The parts are taken in the keys' order within each of the block's warps.
+// Joins the parts of a pair that was cut: block (pair, rows).  Few parts: a warp takes a row alone.  Many, or a block with a single row: all
+// warps take every eighth part of the row and meet.  Eight loads of a lane are under way; the order depends on the shapes alone.
+constexpr int kJoinWarps = 8;
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kThreads) paged_decode_join_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(const DecodeArgs a) {
   using C = Config<D, MT>;
-  __shared__ float sTop[kWarps], sSum[kWarps], sO[kWarps][D];
+  using V = typename std::conditional<D == 128, float4, float2>::type;   // a lane's elements
+  constexpr int kEach = D / 32;
+  extern __shared__ float sF[];                    // [parts]
+  __shared__ float sTop[kJoinWarps], sSum[kJoinWarps], sO[kJoinWarps][D];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const PagedArgs& p = a.p;
-  const int pair = blockIdx.x, b = pair / p.kvHeads, row = blockIdx.y;
+  const int pair = blockIdx.x, b = pair / p.kvHeads, h = pair - b * p.kvHeads;
+  const int2 rec = a.records[pair];                // read before it is known to be one: the workspace holds it in any case
   const Sequence s = sequenceOf(p, b);
-  if (s.n == 0 || (long long)s.n * p.group > C::kRows || row >= s.n * p.group) return;
-  const int2 rec = a.records[pair];
-  if (rec.y < 2) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float* part = a.slots + (((long long)pair + rec.x) * a.slotRows + row) * (D + 2);
-  const long long stride = (long long)a.slotRows * (D + 2);
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < rec.y; i += kThreads) top = fmaxf(top, part[i * stride + D]);
-  top = warpMax(top);
-  if (lane == 0) sTop[warp] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(sTop[0], sTop[1]), fmaxf(sTop[2], sTop[3]));
-  constexpr int kEach = D / 32;
-  float x[kEach], sum = 0.f;
+  const int row0 = blockIdx.y * a.joinRows, rows = s.n * p.group;
+  if (s.n == 0 || (long long)s.n * p.group > C::kRows || row0 >= rows || rec.y < 2) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = rec.y;
+  const long long stride = (long long)a.slotRows * (D + kTail);
+  // Sums the parts first, first + step, ... of a row with factors that `factor` knows.
+  auto add = [&](const float* part, int first, int step, float* x, auto factor) {
+#pragma unroll 1
+    for (int i = first; i < parts; i += 8 * step) {
+      V v[8];
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) x[e] = 0.f;
-#pragma unroll 8
-  for (int i = warp; i < rec.y; i += kWarps) {
-    const float2 ml = *reinterpret_cast<const float2*>(part + i * stride + D);
-    const float f = ml.x == -INFINITY ? 0.f : exp2Fast(ml.x - top);
-    sum += ml.y * f;
+      for (int u = 0; u < 8; ++u) {
+        const int n = i + u * step;
+        if (n < parts) v[u] = reinterpret_cast<const V*>(part + n * stride)[lane];
+      }
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) x[e] = fmaf(part[i * stride + lane + 32 * e], f, x[e]);
+      for (int u = 0; u < 8; ++u) {
+        const int n = i + u * step;
+        const float f = factor(n < parts ? n : i);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+          if (n < parts) x[e] = fmaf(reinterpret_cast<const float*>(&v[u])[e], f, x[e]);
+      }
+    }
+  };
+  auto place = [&](int row) {
+    const int tok = row / p.group;
+    return reinterpret_cast<T*>(p.out) + (s.begin + tok) * p.oSt + (h * p.group + row - tok * p.group) * p.oSh;
+  };
+  if (a.joinRows > 1 && parts <= 32) {
+    const int row = row0 + warp;
+    if (row >= rows) return;
+    const float* part = a.slots + ((long long)pair + rec.x) * stride + row * (D + kTail);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < parts) ml = *reinterpret_cast<const float2*>(part + lane * stride + D);
+    const float top = warpMax(ml.x), f = ml.x == -INFINITY ? 0.f : exp2Fast(ml.x - top), total = warpSum(ml.y * f), inv = total == 0.f ? 0.f : 1.f / total;
+    float x[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) x[e] = 0.f;
+    add(part, 0, 1, x, [&](int n) { return __shfl_sync(0xffffffffu, f, n); });
+    T* dst = place(row) + lane * kEach;
+    if constexpr (kEach == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv));
+    else *reinterpret_cast<uint32_t*>(dst) = pack2<T>(x[0] * inv, x[1] * inv);
+    return;
   }
+  for (int row = row0; row < row0 + a.joinRows && row < rows; ++row) {
+    const float* part = a.slots + ((long long)pair + rec.x) * stride + row * (D + kTail);
+    float top = -INFINITY, sum = 0.f;
+    for (int i = threadIdx.x; i < parts; i += kJoinWarps * 32) top = fmaxf(top, part[i * stride + D]);
+    top = warpMax(top);
+    if (lane == 0) sTop[warp] = top;
+    __syncthreads();
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) sO[warp][lane + 32 * e] = x[e];
-  if (lane == 0) sSum[warp] = sum;
-  __syncthreads();
-  if (threadIdx.x < D) {
-    const float v = (sO[0][threadIdx.x] + sO[1][threadIdx.x]) + (sO[2][threadIdx.x] + sO[3][threadIdx.x]), total = (sSum[0] + sSum[1]) + (sSum[2] + sSum[3]);
-    const int tok = row / p.group, h = pair - b * p.kvHeads;
-    T* dst = reinterpret_cast<T*>(p.out) + (s.begin + tok) * p.oSt + (h * p.group + row - tok * p.group) * p.oSh;
-    const float y = total == 0.f ? 0.f : v / total;
-    if constexpr (std::is_same<T, __half>::value) dst[threadIdx.x] = __float2half_rn(y);
-    else dst[threadIdx.x] = __float2bfloat16_rn(y);
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, sTop[w]);
+    for (int i = threadIdx.x; i < parts; i += kJoinWarps * 32) {
+      const float2 ml = *reinterpret_cast<const float2*>(part + i * stride + D);
+      const float f = ml.x == -INFINITY ? 0.f : exp2Fast(ml.x - top);
+      sF[i] = f;
+      sum += ml.y * f;
+    }
+    sum = warpSum(sum);
+    if (lane == 0) sSum[warp] = sum;
+    __syncthreads();
+    float x[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) x[e] = 0.f;
+    add(part, warp, kJoinWarps, x, [&](int n) { return sF[n]; });
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) sO[warp][lane * kEach + e] = x[e];
+    __syncthreads();
+    if (threadIdx.x < D) {
+      float y = 0.f, total = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) { y += sO[w][threadIdx.x]; total += sSum[w]; }
+      y = total == 0.f ? 0.f : y / total;
+      if constexpr (std::is_same<T, __half>::value) place(row)[threadIdx.x] = __float2half_rn(y);
+      else place(row)[threadIdx.x] = __float2bfloat16_rn(y);
+    }
+    __syncthreads();                               // before the next row's statistics
   }
 }
 
@@ -516,7 +567,7 @@ template <int D, int MT> Launch launchOf(const PagedArgs& p) {
   const long long rows = p.maxQ * p.group;
   Launch l{longest > 512 || pairs > slots, 0, (int)(rows < MT * 16 ? rows : MT * 16), 0};
   l.ctas = (unsigned)(l.split ? slots : pairs);
-  if (l.split) l.bytes = ((pairs * 8 + 15) & ~15LL) + (pairs + slots * kWarps) * l.rows * (D + 2) * 4;
+  if (l.split) l.bytes = ((pairs * 8 + 15) & ~15LL) + (pairs + slots * kWarps) * l.rows * (D + kTail) * 4;
   return l;
 }
 
@@ -551,8 +602,11 @@ int launch(const PagedArgs& p, void* workspace, long long bytes, cudaStream_t st
   a.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((pairs * 8 + 15) & ~15LL));
   if (int rc = launchMain<T, D, MT, true>(mk, mv, a, l.ctas, st)) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)pairs, (unsigned)l.rows);
-  cfg.blockDim = dim3(kThreads);
+  // a row a block while that leaves the SMs with few blocks each: then the parts are many and their sums long
+  a.joinRows = pairs * l.rows <= 8LL * deviceSMs() ? 1 : kJoinWarps;
+  cfg.gridDim = dim3((unsigned)pairs, (unsigned)((l.rows + a.joinRows - 1) / a.joinRows));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.dynamicSmemBytes = l.ctas * kWarps * sizeof(float);   // a pair has at most a part in every warp
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
