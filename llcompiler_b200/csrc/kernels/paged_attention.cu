@@ -140,7 +140,9 @@ bool tensorTypes(const PagedArgs& a) {
 int decodeRows(const PagedArgs& a) {
   const long long rows = a.maxQ * a.group;
   if (rows <= 32) return rows <= 16 ? 16 : 32;
-  if (a.batch == 1) return 0;
+  // few sequences of few keys fit beside the chunks' tiles, and a launch less is worth more (nine sequences of up to 2048 keys, one of them
+  // a single token: 35 us with one kernel, 47 with both)
+  if (a.batch == 1 || (a.reach <= 4096 && a.batch * a.kvHeads <= deviceSMs())) return 0;
   return a.group <= 16 ? 16 : a.group <= 32 ? 32 : 0;
 }
 

@@ -26,6 +26,7 @@ using namespace tc;
 constexpr int kSoftmaxWarps = 16, kLoaderWarp = 16, kIssuerWarp = 17;
 constexpr int kThreads = 20 * 32;          // the last two warps are idle: they fill the warpgroup that gives registers away
 constexpr int kTileRows = 128, kCtaRows = 256, kKeys = 128;
+constexpr int kCutBlocks = 12;            // least blocks of a part (nine sequences of up to 2048 keys: 59 us with 2, 35 with 12)
 constexpr int kMaxSplits = 32;
 
 template <int D> struct Config {
@@ -43,10 +44,11 @@ constexpr uint32_t kColS = 0, kColO = 256;
 struct ChunkArgs {
   PagedArgs p;
   int doneRows;                // sequences of at most so many rows are the decode kernel's
-  int pageShift, boxRows, splits;
+  int pageShift, boxRows;
+  int maxCut, maxSplits;       // CTAs that cut keys may fill, one and a half times the SMs (0: no key is cut), most parts of a tile's keys
   float scaleAbs, signQ;       // the scale's size; its sign goes into Q, so that the largest product is the largest score
-  int4* records;               // [tiles * key heads]: sequence (or -1) and first row of each pair of tiles
-  float* parts;                // [tiles * key heads][2][splits][kPart]
+  int4* records;               // [0]: pairs of tiles of the call, parts of each; then of each pair its sequence and tile
+  float* parts;                // [pairs][2][parts][kPart]
 };
 
 // What a tile's rows see.
@@ -97,6 +99,7 @@ struct Plan {
   Seen seen;                   // by the rows of both
   int begin, end;              // units of this CTA's part of the keys
   int seq, tile;               // sequence (-1: nothing to do) and pair of tiles
+  int pair, split, splits;     // (pair of tiles, key head), which part of its keys of how many
   int n, len;                  // of the sequence
   int row0, rows, qBegin;      // rows (token, query head) of the sequence: the host keeps tokens x query heads below 2^31
 };
@@ -224,14 +227,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
   if (smemAddr(smem) & 1023) {                        // the swizzled tiles need it; no static shared memory lies before them
     if (threadIdx.x == 0) {
       atomicExch(&g_pagedChunkStatus, 10);
-      if (a.splits > 1 && blockIdx.x % a.splits == 0) a.records[(long long)blockIdx.y * p.kvHeads + blockIdx.x / a.splits] = make_int4(-1, 0, 0, 0);
+      if (a.maxCut && blockIdx.x == 0) a.records[0] = make_int4(0, 1, 0, 0);
     }
     return;
   }
 
-  // Which sequence and tiles: blockIdx.x = head and part of the keys, blockIdx.y = tile pair, counted from the last, which sees the
-  // most keys of its sequence.
-  const int h = blockIdx.x / a.splits, split = blockIdx.x - h * a.splits;
+  asm volatile("griddepcontrol.launch_dependents;");
+  // Which sequence and tiles.  The pairs of tiles, heads of one pair side by side, are taken from the last, which sees the most keys of its
+  // sequence.  Where they leave SMs idle (known here, from the lengths), each is cut into parts of its keys.
+  int h;
   {
     // a thread keeps its (last) sequence: with up to kThreads of them nothing is read twice
     const int per = (p.batch + kThreads - 1) / kThreads, first = threadIdx.x * per;
@@ -254,7 +258,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     int before = run - mine, all = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) { const int x = sScan[w]; if (w < warp) before += x; all += x; }
-    const int want = all - 1 - (int)blockIdx.y;
+    const long long pairs = (long long)all * p.kvHeads;
+    int splits = 1;
+    if (pairs > 0 && 2 * pairs <= a.maxCut) splits = min((2 * a.maxCut / 3 + (int)pairs / 2) / (int)pairs, a.maxSplits);   // nearest to the SMs
+    if (a.maxCut && blockIdx.x == 0 && threadIdx.x == 0) a.records[0] = make_int4((int)min(pairs, 0x7fffffffLL), splits, 0, 0);
+    const int pair = blockIdx.x / (unsigned)splits, split = blockIdx.x - pair * splits, tile = pair / p.kvHeads;
+    h = pair - tile * p.kvHeads;
+    const int want = all - 1 - tile;
     if (want >= before && want < before + mine) {
       int i = first;
       if (per > 1) {
@@ -269,7 +279,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
       const Tile tile0 = tileOf(p, s, row0, rows), tile1 = tileOf(p, s, row0 + kTileRows, rows);
       plan->seen = seenBy(p, tile0.first, tile1.last >= 0 ? tile1.last : tile0.last);
       const Blocks bl = blocksOf(plan->seen, kKeys);
-      const int share = (bl.count + a.splits - 1) / a.splits, begin = share * split < bl.count ? share * split : bl.count;
+      const int share = (bl.count + splits - 1) / splits, begin = share * split < bl.count ? share * split : bl.count;
       plan->units[0] = unitsOf(p, tile0, bl);
       plan->units[1] = unitsOf(p, tile1, bl);
       plan->bl = bl;
@@ -277,11 +287,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
       plan->end = begin + share < bl.count ? begin + share : bl.count;
       plan->seq = i; plan->tile = want - before; plan->n = s.n; plan->len = s.len;
       plan->row0 = row0; plan->rows = rows; plan->qBegin = (int)s.begin;
+      plan->pair = pair; plan->split = split; plan->splits = splits;
+      if (splits > 1 && split == 0) a.records[1 + pair] = make_int4(i, want - before, 0, 0);
     }
     __syncthreads();
   }
-  const long long pair = (long long)blockIdx.y * p.kvHeads + h;
-  if (a.splits > 1 && split == 0 && threadIdx.x == 0) a.records[pair] = make_int4(plan->seq, plan->tile, 0, 0);
   if (plan->seq < 0) return;                          // fewer tiles than the grid has room for
   if (warp == kIssuerWarp) tmemAlloc(tmemSlot, 512);
   tcFenceBefore();
@@ -575,8 +585,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     pairBarrier(bar);
     l += loadShared(otherAt);
     const float base = m == -INFINITY ? 0.f : m - kShift;
-    const bool cut = a.splits > 1;
-    float* part = a.parts + ((pair * 2 + t) * a.splits + split) * C::kPart;
+    const bool cut = plan->splits > 1;
+    float* part = a.parts + (((long long)plan->pair * 2 + t) * plan->splits + plan->split) * C::kPart;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     bool odd = false;
     if (cut && side == 0) {
@@ -658,16 +668,16 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const ChunkArgs a
   __shared__ float sF[kMaxSplits][kTileRows];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const PagedArgs& p = a.p;
-  const long long pair = blockIdx.x >> 1;
-  const int t = blockIdx.x & 1, r = threadIdx.x & 127, side = threadIdx.x >> 7;
-  const int4 rec = a.records[pair];
-  if (rec.x < 0) return;
+  const int4 call = a.records[0];
+  const int pair = blockIdx.x >> 1, t = blockIdx.x & 1, r = threadIdx.x & 127, side = threadIdx.x >> 7, splits = call.y;
+  if (splits < 2 || pair >= call.x) return;
+  const int4 rec = a.records[1 + pair];
   const Sequence s = sequenceOf(p, rec.x);
   const long long rows = (long long)s.n * p.group, row = (long long)rec.y * kCtaRows + t * kTileRows + r;
-  const float* part = a.parts + (pair * 2 + t) * a.splits * C::kPart;
+  const float* part = a.parts + ((long long)pair * 2 + t) * splits * C::kPart;
   float top = -INFINITY, sum = 0.f;
-  for (int i = 0; i < a.splits; ++i) top = fmaxf(top, part[(long long)i * C::kPart + kTileRows * D + r]);
-  for (int i = 0; i < a.splits; ++i) {
+  for (int i = 0; i < splits; ++i) top = fmaxf(top, part[(long long)i * C::kPart + kTileRows * D + r]);
+  for (int i = 0; i < splits; ++i) {
     const float m = part[(long long)i * C::kPart + kTileRows * D + r], l = part[(long long)i * C::kPart + kTileRows * (D + 1) + r];
     const float f = m == -INFINITY ? 0.f : exp2Fast(m - top);
     if (side == 0) sF[i][r] = f;
@@ -682,7 +692,7 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const ChunkArgs a
   for (int c = side; c < D / 4; c += 2) {
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = 0; i < a.splits; ++i) {
+    for (int i = 0; i < splits; ++i) {
       const float f = sF[i][r];
       if (f != 0.f) {                                 // a part that saw nothing may hold anything
         const float4 v = *reinterpret_cast<const float4*>(part + (long long)i * C::kPart + ((long long)c * kTileRows + r) * 4);
@@ -693,27 +703,22 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const ChunkArgs a
   }
 }
 
-// Pairs of tiles that the grid has room for (a bound from what the host knows), and in how many parts the keys are taken: one where
-// the pairs alone fill the SMs, else as many as bring the grid to one CTA an SM, at least two blocks of keys each.
-struct Launch { long long tiles; int splits; };
+// CTAs of the grid (a bound on the pairs of tiles times key heads from what the host knows), and whether keys may be cut: where the rows that
+// the call names would fill less than three quarters of the SMs, and enough
+// blocks of keys are left to each part: a part costs a CTA's start and end and its sums' way through memory, what eight blocks cost.
+struct Launch { long long ctas; int maxCut, maxSplits; };
 Launch launchOf(const PagedArgs& p) {
-  Launch l;
-  const long long each = (p.maxQ * p.group + kCtaRows - 1) / kCtaRows, most = p.tokens * p.group / kCtaRows + p.batch;
-  l.tiles = each * p.batch < most ? each * p.batch : most;
-  const long long ctas = l.tiles * p.kvHeads, sms = deviceSMs();
+  Launch l{};
+  const long long each = (p.maxQ * p.group + kCtaRows - 1) / kCtaRows, most = p.tokens * p.group / kCtaRows + p.batch, sms = deviceSMs();
+  l.ctas = (each * p.batch < most ? each * p.batch : most) * p.kvHeads;
   long long longest = p.reach;
   if ((long long)p.window + p.sinks + kCtaRows < longest) longest = (long long)p.window + p.sinks + kCtaRows;
-  long long splits = ctas >= sms ? 1 : sms / ctas;
-  const long long most2 = (longest + 2 * kKeys - 1) / (2 * kKeys);
-  if (splits > most2) splits = most2;
-  if (splits > kMaxSplits) splits = kMaxSplits;
-  l.splits = splits < 1 ? 1 : (int)splits;
+  const long long splits = longest / (kCutBlocks * kKeys);
+  l.maxSplits = (int)(splits < kMaxSplits ? splits : kMaxSplits);
+  if (l.maxSplits > 1 && 4 * (p.tokens * p.group / kCtaRows) * p.kvHeads <= 3 * sms) l.maxCut = (int)(sms * 3 / 2);
   return l;
 }
-template <int D> long long bytesOf(const PagedArgs& p, const Launch& l) {
-  const long long pairs = l.tiles * p.kvHeads;
-  return l.splits == 1 ? 0 : pairs * 16 + pairs * 2 * l.splits * Config<D>::kPart * 4;
-}
+template <int D> long long bytesOf(const Launch& l) { return l.maxCut ? 16LL * (1 + l.maxCut) + 2LL * l.maxCut * Config<D>::kPart * 4 : 0; }
 
 template <typename T, int D>
 int launch(const PagedArgs& p, int doneRows, void* workspace, long long bytes, cudaStream_t st) {
@@ -730,23 +735,24 @@ int launch(const PagedArgs& p, int doneRows, void* workspace, long long bytes, c
   a.scaleAbs = fabsf(p.scaleLog2) > 1e-37f || p.scaleLog2 != p.scaleLog2 ? fabsf(p.scaleLog2) : 1e-37f;
   a.signQ = p.scaleLog2 < 0.f ? -1.f : 1.f;
   Launch l = launchOf(p);
-  if (!workspace || bytes < bytesOf<D>(p, l)) l.splits = 1;
-  a.splits = l.splits;
-  const long long pairs = l.tiles * p.kvHeads;
+  if (!workspace || bytes < bytesOf<D>(l)) l.maxCut = 0;
+  if (l.ctas < l.maxCut) l.ctas = l.maxCut;
+  if (l.ctas > 0x7FFFFFFFLL) return setError(LLC_ERR_UNSUPPORTED, "llc argument: paged_attention too many tiles");
+  a.maxCut = l.maxCut;
+  a.maxSplits = l.maxSplits;
   a.records = static_cast<int4*>(workspace);
-  a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + pairs * 16);
-  if (l.tiles > 65535 || (long long)p.kvHeads * l.splits > 0x7FFFFFFFLL) return setError(LLC_ERR_UNSUPPORTED, "llc argument: paged_attention too many tiles");
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + 16LL * (1 + l.maxCut));
   static DeviceOnce configured;
   const int dev = currentDevice();
   if (!configured.test(dev)) {
     LLC_CUDA_CHECK(cudaFuncSetAttribute(paged_chunk_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     configured.set(dev);
   }
-  paged_chunk_kernel<T, D><<<dim3((unsigned)(p.kvHeads * l.splits), (unsigned)l.tiles), kThreads, C::kSmem, st>>>(mk, mv, a);
+  paged_chunk_kernel<T, D><<<(unsigned)l.ctas, kThreads, C::kSmem, st>>>(mk, mv, a);
   LLC_LAUNCH_CHECK("paged_chunk_kernel");
-  if (l.splits > 1) {
+  if (l.maxCut) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(2 * pairs));
+    cfg.gridDim = dim3((unsigned)l.maxCut);         // two tiles of each of at most maxCut / 2 pairs
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -762,7 +768,7 @@ int launch(const PagedArgs& p, int doneRows, void* workspace, long long bytes, c
 }  // namespace
 
 // The sequences of more than doneRows rows (new tokens x query heads of a key head).
-long long pagedChunkWorkspace(const PagedArgs& p) { return p.d == 64 ? bytesOf<64>(p, launchOf(p)) : bytesOf<128>(p, launchOf(p)); }
+long long pagedChunkWorkspace(const PagedArgs& p) { return p.d == 64 ? bytesOf<64>(launchOf(p)) : bytesOf<128>(launchOf(p)); }
 int pagedChunk(const PagedArgs& p, int doneRows, void* workspace, long long bytes, cudaStream_t st) {
   if (p.dtype == LLC_BFLOAT16)
     return p.d == 64 ? launch<__nv_bfloat16, 64>(p, doneRows, workspace, bytes, st) : launch<__nv_bfloat16, 128>(p, doneRows, workspace, bytes, st);

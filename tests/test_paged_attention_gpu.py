@@ -53,6 +53,14 @@ CASES = [
     ([90], [300], 4, 1, 128, 16, 60, 140),
     ([12, 300], [5, 290], 2, 2, 64, 16, 0, 0),               # more new tokens than keys: the first ones see nothing
     ([64], [1000], 16, 1, 128, 256, 0, 0),
+    # keys cut into parts: of chunks (at least 1536 keys each) and of few rows (each warp its share)
+    ([20], [5000], 2, 1, 128, 64, 0, 0),
+    ([40], [5000], 2, 2, 64, 16, 0, 0),
+    ([17, 1, 35], [4001, 4999, 60], 2, 1, 64, 32, 0, 0),
+    ([36], [6500], 1, 1, 64, 16, 4700, 9),
+    ([1], [5000], 2, 1, 128, 16, 0, 0),
+    ([3, 1], [4100, 7], 4, 2, 64, 128, 0, 0),
+    ([7], [2100], 4, 1, 128, 16, 1900, 50),
 ]
 
 
@@ -94,7 +102,8 @@ def test_scores_that_grow_shrink_and_overflow_the_running_maximum(new, lens):
         _check(got, q, k, v, table, q_start, kv_len, scale=scale)
 
 
-@pytest.mark.parametrize("new,lens,window,sinks", [([1, 1], [300, 170], 40, 3), ([60, 2], [300, 170], 40, 3), ([1, 40], [90, 64], 0, 0)])
+@pytest.mark.parametrize("new,lens,window,sinks", [([1, 1], [300, 170], 40, 3), ([60, 2], [300, 170], 40, 3), ([1, 40], [90, 64], 0, 0), ([3, 2], [300, 60], 0, 0),
+                                                   ([4, 1], [900, 30], 20, 2), ([30, 1], [5000, 30], 3600, 3)])
 @pytest.mark.parametrize("what", [float("nan"), float("inf"), float("-inf")])
 def test_keys_that_are_not_visible_may_hold_anything(new, lens, window, sinks, what):
     """Keys that no token of the call sees hold NaN and infinities (they lie before the window, behind the sinks), and a
@@ -243,6 +252,33 @@ def test_captured_step_replays_with_other_lengths():
         torch.cuda.synchronize()
         for s, (out, q) in zip(steps, outs):
             _check(out, q.cpu(), s.kc.cpu(), s.vc.cpu(), table, q_start, s.kv_len.cpu())
+
+
+def test_one_long_sequence_among_many_short_ones():
+    """More (sequence, key head, row) sums than the joining kernel gives a block each, one pair cut into many parts, and the same
+    without a workspace."""
+    import ctypes
+    from llcompiler_b200 import _capi as C
+    batch, heads, kv_heads, d, page = 80, 16, 4, 64, 16
+    lens = [17] * batch
+    lens[37] = 6000
+    k, v, table, q_start, kv_len = R.make_batch([1] * batch, lens, page, kv_heads, d, torch.bfloat16)
+    q = _q(batch, heads, d, torch.bfloat16)
+    got = _run(q, k, v, table, q_start, kv_len, max_q=1)
+    _check(got, q, k, v, table, q_start, kv_len)
+    dev = [R.to_device(t, DEV) for t in (q, k, v, table, q_start, kv_len)]
+    out = torch.full(q.shape, 5.0, device=DEV, dtype=torch.bfloat16)
+    p = C.LlcPagedAttentionParams()
+    p.q, p.k_cache, p.v_cache, p.page_table, p.q_start, p.kv_len = (ctypes.c_void_p(t.data_ptr()) for t in dev)
+    p.out, p.dtype, p.scale = ctypes.c_void_p(out.data_ptr()), 8, R.scale_of(d)
+    p.tokens, p.batch, p.heads, p.kv_heads, p.d, p.max_q = batch, batch, heads, kv_heads, d, 1
+    p.num_pages, p.page_size, p.table_width, p.table_s0 = k.shape[0], page, table.shape[1], table.stride(0)
+    p.q_st, p.q_sh, p.o_st, p.o_sh = q.stride(0), q.stride(1), out.stride(0), out.stride(1)
+    p.kc_sp, p.kc_sn, p.kc_sh = k.stride()[:3]
+    p.vc_sp, p.vc_sn, p.vc_sh = v.stride()[:3]
+    assert C.lib().llc_cuda_paged_attention_workspace(ctypes.byref(p)) > 0
+    C.check(C.lib().llc_cuda_paged_attention(ctypes.byref(p), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    _check(out, q, k, v, table, q_start, kv_len)
 
 
 def test_other_streams():
