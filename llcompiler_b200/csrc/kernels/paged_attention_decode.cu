@@ -565,7 +565,9 @@ template <int D, int MT> Launch launchOf(const PagedArgs& p) {
   long long longest = p.reach;                     // keys that a sequence can see
   if ((long long)p.window + p.sinks + MT * 16 < longest) longest = (long long)p.window + p.sinks + MT * 16;
   const long long rows = p.maxQ * p.group;
-  Launch l{longest > 512 || pairs > slots, 0, (int)(rows < MT * 16 ? rows : MT * 16), 0};
+  // a CTA a pair: up to 512 keys each, and no more work than one such pair a CTA, in at most two rounds of CTAs
+  const bool whole = longest <= 512 && pairs <= 2 * slots && pairs * longest <= 512 * slots;
+  Launch l{!whole, 0, (int)(rows < MT * 16 ? rows : MT * 16), 0};
   l.ctas = (unsigned)(l.split ? slots : pairs);
   if (l.split) l.bytes = ((pairs * 8 + 15) & ~15LL) + (pairs + slots * kWarps) * l.rows * (D + kTail) * 4;
   return l;

@@ -170,7 +170,7 @@ struct Execution {
 struct Torch {
   py::object tensor, emptyLike, empty, stream, gradEnabled;
   py::object f32, f16, bf16, f64, i32, i64;
-  PyObject* nShape, *nStride, *nDtype, *nPtr, *nDevice, *nGrad;
+  PyObject* nShape, *nStride, *nDtype, *nPtr, *nDevice, *nGrad, *nDeviceOf, *kwEmpty;
   Torch() {
     py::module_ t = py::module_::import("torch"), c = py::module_::import("torch._C");
     tensor = t.attr("Tensor"); emptyLike = t.attr("empty_like"); empty = t.attr("empty"); gradEnabled = t.attr("is_grad_enabled");
@@ -178,6 +178,8 @@ struct Torch {
     f32 = t.attr("float32"); f16 = t.attr("float16"); bf16 = t.attr("bfloat16"); f64 = t.attr("float64"); i32 = t.attr("int32"); i64 = t.attr("int64");
     nShape = PyUnicode_InternFromString("shape"); nStride = PyUnicode_InternFromString("stride"); nDtype = PyUnicode_InternFromString("dtype");
     nPtr = PyUnicode_InternFromString("data_ptr"); nDevice = PyUnicode_InternFromString("get_device"); nGrad = PyUnicode_InternFromString("requires_grad");
+    nDeviceOf = PyUnicode_InternFromString("device");
+    kwEmpty = PyTuple_Pack(2, nDtype, nDeviceOf);
   }
   int code(PyObject* d) const {
     if (d == bf16.ptr()) return LLC_BFLOAT16;
@@ -193,6 +195,12 @@ const Torch& torch() { static Torch* t = new Torch(); return *t; }   // never de
 
 py::object got(PyObject* o) { if (!o) throw py::error_already_set(); return py::reinterpret_steal<py::object>(o); }
 
+int64_t number(const char* name, PyObject* o) {
+  const long long x = PyLong_AsLongLong(o);
+  if (x == -1 && PyErr_Occurred()) { PyErr_Clear(); throw py::type_error(std::string(name) + ": expected a whole number of 64 bits"); }
+  return x;
+}
+
 // One operand.  `name` goes into the message when something does not fit.
 struct Operand {
   const char* name;
@@ -205,12 +213,13 @@ struct Operand {
     for (int i = 0; i < rank; ++i) r += (i ? ", " : "") + std::to_string(n[i]);
     return r + ")";
   }
-  Operand(const char* name_, py::handle h, int least, int most) : name(name_) {
+  // The caller's tensor, checked.  Whole numbers never require a gradient: `index` skips that question.
+  Operand(const char* name_, py::handle h, int least, int most, bool index = false) : name(name_) {
     const Torch& t = torch();
     PyObject* o = h.ptr();
     if (!PyObject_TypeCheck(o, reinterpret_cast<PyTypeObject*>(t.tensor.ptr()))) throw py::type_error(std::string(name) + ": expected a tensor, got " + Py_TYPE(o)->tp_name);
     py::object sh = got(PyObject_GetAttr(o, t.nShape)), st = got(PyObject_CallMethodNoArgs(o, t.nStride)), dt = got(PyObject_GetAttr(o, t.nDtype)),
-               dv = got(PyObject_CallMethodNoArgs(o, t.nDevice)), gr = got(PyObject_GetAttr(o, t.nGrad)), pt = got(PyObject_CallMethodNoArgs(o, t.nPtr));
+               dv = got(PyObject_CallMethodNoArgs(o, t.nDevice)), pt = got(PyObject_CallMethodNoArgs(o, t.nPtr));
     rank = (int)PyTuple_GET_SIZE(sh.ptr());
     if (rank < least || rank > most) throw py::value_error(std::string(name) + ": expected " + std::to_string(least) + " dims, got " + std::to_string(rank));
     for (int i = 0; i < rank; ++i) { n[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(sh.ptr(), i)); s[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(st.ptr(), i)); }
@@ -219,7 +228,16 @@ struct Operand {
     ptr = (uintptr_t)PyLong_AsUnsignedLongLong(pt.ptr());
     if (PyErr_Occurred()) throw py::error_already_set();
     if (device < 0) bad("expected a CUDA tensor; there is no CPU fallback");
-    if (gr.ptr() == Py_True && t.gradEnabled().cast<bool>()) bad("inference only, it requires a gradient");
+    if (!index && got(PyObject_GetAttr(o, t.nGrad)).ptr() == Py_True && t.gradEnabled().cast<bool>()) bad("inference only, it requires a gradient");
+  }
+  // A tensor just made like `l`: only its strides and its address are news.
+  Operand(const char* name_, py::handle h, const Operand& l) : name(name_) {
+    const Torch& t = torch();
+    py::object st = got(PyObject_CallMethodNoArgs(h.ptr(), t.nStride)), pt = got(PyObject_CallMethodNoArgs(h.ptr(), t.nPtr));
+    rank = l.rank; dtype = l.dtype; device = l.device;
+    for (int i = 0; i < rank; ++i) { n[i] = l.n[i]; s[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(st.ptr(), i)); }
+    ptr = (uintptr_t)PyLong_AsUnsignedLongLong(pt.ptr());
+    if (PyErr_Occurred()) throw py::error_already_set();
   }
   void on(int dev) const { if (device != dev) bad("on cuda:" + std::to_string(device) + ", expected cuda:" + std::to_string(dev)); }
   void type(int want, const char* said) const { if (dtype != want) bad(std::string("expected ") + said); }
@@ -242,8 +260,8 @@ Operand firstRows(const char* name, py::handle h) {
 Operand output(const char* name, py::object& out, py::handle like, const Operand& l) {
   const bool own = out.is_none();
   if (own) {
-    out = torch().emptyLike(like);
-    Operand o(name, out, 3, 3);
+    out = got(PyObject_CallOneArg(torch().emptyLike.ptr(), like.ptr()));
+    Operand o(name, out, l);
     if (l.n[2] <= 1 || o.s[2] == 1) return o;
     out = torch().empty(like.attr("shape"), py::arg("dtype") = like.attr("dtype"), py::arg("device") = like.attr("device"));
   }
@@ -258,7 +276,7 @@ Operand output(const char* name, py::object& out, py::handle like, const Operand
 struct Turns { uintptr_t positions = 0, freq = 0; int posType = LLC_INT64, axes = 0; int64_t posStride = 0, pairs = 0; int32_t sections[LLC_ROTARY_MAX_AXES] = {0, 0, 0, 0}; };
 Turns turns(py::handle positions, py::handle freq, py::handle sections, int64_t tokens, int64_t d, int device) {
   Turns t;
-  Operand f("inv_freq", freq, 1, 1);
+  Operand f("inv_freq", freq, 1, 1, true);
   f.on(device);
   f.type(LLC_FLOAT64, "float64");
   f.unit(0, "it");
@@ -283,7 +301,7 @@ Turns turns(py::handle positions, py::handle freq, py::handle sections, int64_t 
     t.axes = (int)n;
   }
   if (positions.is_none()) return t;
-  Operand p("positions", positions, 1, 2);
+  Operand p("positions", positions, 1, 2, true);
   p.on(device);
   if (p.dtype != LLC_INT32 && p.dtype != LLC_INT64) p.bad("expected int32 or int64");
   const int last = p.rank - 1;
@@ -295,13 +313,13 @@ Turns turns(py::handle positions, py::handle freq, py::handle sections, int64_t 
 
 struct Batch { int64_t size, width, stride; const int32_t *table, *start, *len; int32_t* bad; };
 Batch batchOf(py::handle table, py::handle start, py::handle len, py::handle bad, int device) {
-  Operand t("page_table", table, 2, 2), s("q_start", start, 1, 1), l("kv_len", len, 1, 1);
+  Operand t("page_table", table, 2, 2, true), s("q_start", start, 1, 1, true), l("kv_len", len, 1, 1, true);
   for (const Operand* o : {&t, &s, &l}) { o->on(device); o->type(LLC_INT32, "int32"); o->unit(o->rank - 1, "the last dim"); }
   if (s.n[0] != t.n[0] + 1) s.bad("expected " + std::to_string(t.n[0] + 1) + " entries, got " + std::to_string(s.n[0]));
   if (l.n[0] != t.n[0]) l.bad("expected " + std::to_string(t.n[0]) + " entries, got " + std::to_string(l.n[0]));
   Batch b{t.n[0], t.n[1], t.s[0], reinterpret_cast<const int32_t*>(t.ptr), reinterpret_cast<const int32_t*>(s.ptr), reinterpret_cast<const int32_t*>(l.ptr), nullptr};
   if (!bad.is_none()) {
-    Operand x("bad_pages", bad, 1, 1);
+    Operand x("bad_pages", bad, 1, 1, true);
     x.on(device);
     x.type(LLC_INT32, "int32");
     if (x.n[0] != 1) x.bad("expected one counter");
@@ -320,7 +338,10 @@ Operand cacheOf(const char* name, py::handle h, const Operand& first) {
 void sameShape(const Operand& a, const Operand& b) {
   for (int i = 0; i < a.rank; ++i) if (a.n[i] != b.n[i]) b.bad("expected shape " + a.shape() + ", got " + b.shape());
 }
-void* streamOf(int device) { return reinterpret_cast<void*>(torch().stream(device).cast<uintptr_t>()); }
+void* streamOf(int device) {
+  py::object d = got(PyLong_FromLong(device)), s = got(PyObject_CallOneArg(torch().stream.ptr(), d.ptr()));
+  return PyLong_AsVoidPtr(s.ptr());
+}
 template <typename T = void> T* at(uintptr_t p) { return reinterpret_cast<T*>(p); }
 
 py::object rotary(py::handle x, py::handle positions, py::handle freq, py::handle sections, bool interleaved, py::object out) {
@@ -376,12 +397,12 @@ py::object pagedAttention(py::handle q, py::handle kCache, py::handle vCache, py
   if (a.n[2] != d || a.n[1] == 0 || a.n[1] % kv) a.bad("expected [tokens, a multiple of " + std::to_string(kv) + ", " + std::to_string(d) + "], got " + a.shape());
   const Batch s = batchOf(table, start, len, bad, a.device);
   if (window < 0 || sinks < 0) throw py::value_error("window and sinks: must not be negative");
-  const int64_t most = maxQ.is_none() ? a.n[0] : maxQ.cast<int64_t>();
+  const int64_t most = maxQ.is_none() ? a.n[0] : number("max_q", maxQ.ptr());
   if (most < 0) throw py::value_error("max_q: must not be negative");
   const Operand o = output("out", out, q, a);
   LlcPagedAttentionParams p{};
   p.q = at(a.ptr); p.k_cache = at(kc.ptr); p.v_cache = at(vc.ptr); p.out = at(o.ptr); p.page_table = s.table; p.q_start = s.start; p.kv_len = s.len; p.bad_pages = s.bad;
-  p.dtype = a.dtype; p.scale = scale.is_none() ? (float)(1.0 / std::sqrt((double)d)) : scale.cast<float>();
+  p.dtype = a.dtype; p.scale = scale.is_none() ? (float)(1.0 / std::sqrt((double)d)) : (float)py::float_(scale);
   p.tokens = a.n[0]; p.batch = s.size; p.heads = a.n[1]; p.kv_heads = kv; p.d = d; p.max_q = most; p.num_pages = kc.n[0]; p.page_size = kc.n[1];
   p.table_width = s.width; p.table_s0 = s.stride; p.window = window; p.sinks = sinks;
   p.q_st = a.s[0]; p.q_sh = a.s[1]; p.o_st = o.s[0]; p.o_sh = o.s[1];
@@ -389,13 +410,52 @@ py::object pagedAttention(py::handle q, py::handle kCache, py::handle vCache, py
   // scratch from the caching allocator at every call: ordered with the stream, and a captured graph gets memory of its own
   py::object scratch;
   if (const int64_t bytes = llc_cuda_paged_attention_workspace(&p)) {
-    scratch = torch().empty((bytes + 3) / 4, py::arg("dtype") = torch().f32, py::arg("device") = q.attr("device"));
-    p.workspace = at(scratch.attr("data_ptr")().cast<uintptr_t>());
+    const Torch& t = torch();
+    py::object n = got(PyLong_FromLongLong((bytes + 3) / 4)), dev = got(PyObject_GetAttr(q.ptr(), t.nDeviceOf));
+    PyObject* const args[] = {n.ptr(), t.f32.ptr(), dev.ptr()};
+    scratch = got(PyObject_Vectorcall(t.empty.ptr(), args, 1, t.kwEmpty));
+    p.workspace = at(PyLong_AsUnsignedLongLong(got(PyObject_CallMethodNoArgs(scratch.ptr(), t.nPtr)).ptr()));
     p.workspace_bytes = bytes;
   }
   check(llc_cuda_paged_attention(&p, streamOf(a.device)));
   return out;
 }
+
+// The three as plain functions of the interpreter (positional arguments, a fixed number of them): its own calling convention costs a tenth of
+// a wrapped function's.  C++ exceptions end here.
+template <Py_ssize_t N, typename F> PyObject* enter(const char* name, Py_ssize_t n, F f) {
+  try {
+    if (n != N) throw py::type_error(std::string(name) + ": expected " + std::to_string(N) + " arguments, got " + std::to_string(n));
+    return f().release().ptr();
+  } catch (py::error_already_set& e) {
+    e.restore();
+  } catch (const py::builtin_exception& e) {
+    e.set_error();
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  }
+  return nullptr;
+}
+py::object own(PyObject* o) { return py::reinterpret_borrow<py::object>(o); }
+bool truth(PyObject* o) {
+  const int x = PyObject_IsTrue(o);
+  if (x < 0) throw py::error_already_set();
+  return x != 0;
+}
+PyObject* rotaryEntry(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return enter<6>("rotary", n, [&] { return rotary(a[0], a[1], a[2], a[3], truth(a[4]), own(a[5])); });
+}
+PyObject* kvAppendEntry(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return enter<14>("kv_append", n, [&] { return kvAppend(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], truth(a[11]), own(a[12]), a[13]); });
+}
+PyObject* pagedEntry(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return enter<12>("paged_attention", n, [&] {
+    return pagedAttention(a[0], a[1], a[2], a[3], a[4], a[5], own(a[6]), number("window", a[7]), number("sinks", a[8]), own(a[9]), own(a[10]), a[11]);
+  });
+}
+PyMethodDef kOps[] = {{"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&rotaryEntry)), METH_FASTCALL, nullptr},
+                      {"kv_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&kvAppendEntry)), METH_FASTCALL, nullptr},
+                      {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&pagedEntry)), METH_FASTCALL, nullptr}};
 
 }  // namespace
 
@@ -449,8 +509,6 @@ PYBIND11_MODULE(llcompiler_, m) {
       .def("num_inputs", &Execution::num_inputs).def("num_outputs", &Execution::num_outputs).def("num_symbols", &Execution::num_symbols)
       .def("last_launch_count", &Execution::last_launch_count).def("arena_bytes", &Execution::arena_bytes);
   auto ops = m.def_submodule("ops");
-  ops.def("rotary", &rotary);
-  ops.def("kv_append", &kvAppend);
-  ops.def("paged_attention", &pagedAttention);
+  for (PyMethodDef& f : kOps) ops.attr(f.ml_name) = got(PyCFunction_NewEx(&f, nullptr, nullptr));
   m.def("version", []() { return std::string(llc_version()); });
 }

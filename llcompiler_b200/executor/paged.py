@@ -29,11 +29,11 @@ except ImportError as e:  # the CUDA path is the only path: fail loudly
 _current = torch._C._cuda_getDevice
 
 
-def _call(f, first, *args):
-    """Runs `f` with the first operand's device current; `f` makes the checks and launches on that device's current stream."""
+def _elsewhere(f, first, *args):
+    """Runs `f`, which makes the checks and launches, with the first operand's device current."""
     index = first.get_device() if isinstance(first, torch.Tensor) else -1
-    if index < 0 or index == _current():
-        return f(first, *args)
+    if index < 0:
+        return f(first, *args)      # which refuses it
     with torch.cuda.device(index):
         return f(first, *args)
 
@@ -46,7 +46,9 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sec
     ``sections`` says how many pairs belong to each axis, in order (time, height, width of a video, say; default: one axis).
     Pair i is elements ``(i, i + pairs)``, or ``(2i, 2i + 1)`` when ``interleaved``; elements past the pairs are copied.
     ``out`` may be ``x`` itself."""
-    return _call(_ops.rotary, x, positions, inv_freq, sections, interleaved, out)
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.get_device() == _current():
+        return _ops.rotary(x, positions, inv_freq, sections, interleaved, out)
+    return _elsewhere(_ops.rotary, x, positions, inv_freq, sections, interleaved, out)
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
@@ -59,7 +61,9 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     sequences), and so are the queries ``q [tokens, heads, head_dim]``, which are returned (``q_out``, or a new tensor; rows
     of no sequence are not written).  A token whose page number is no page of the pool, or whose place lies outside the
     table, is not stored and is counted in ``bad_pages`` (one int32) if that is given.  Two tokens must not share a slot."""
-    return _call(_ops.kv_append, k, v, k_cache, v_cache, page_table, q_start, kv_len, q, positions, inv_freq, sections, interleaved, q_out, bad_pages)
+    if isinstance(k, torch.Tensor) and k.is_cuda and k.get_device() == _current():
+        return _ops.kv_append(k, v, k_cache, v_cache, page_table, q_start, kv_len, q, positions, inv_freq, sections, interleaved, q_out, bad_pages)
+    return _elsewhere(_ops.kv_append, k, v, k_cache, v_cache, page_table, q_start, kv_len, q, positions, inv_freq, sections, interleaved, q_out, bad_pages)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
@@ -73,4 +77,6 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     which lets the call choose the kernel for few rows; a sequence that has more is left out.  A token that sees nothing gets
     zeros; rows of no sequence are not written.  Pages that are none of the pool's read as zeros and are counted in
     ``bad_pages`` (one int32) if that is given."""
-    return _call(_ops.paged_attention, q, k_cache, v_cache, page_table, q_start, kv_len, scale, window, sinks, max_q, out, bad_pages)
+    if isinstance(q, torch.Tensor) and q.is_cuda and q.get_device() == _current():
+        return _ops.paged_attention(q, k_cache, v_cache, page_table, q_start, kv_len, scale, window, sinks, max_q, out, bad_pages)
+    return _elsewhere(_ops.paged_attention, q, k_cache, v_cache, page_table, q_start, kv_len, scale, window, sinks, max_q, out, bad_pages)
