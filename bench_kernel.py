@@ -11,7 +11,10 @@ command that profiler captures are taken on, and the per-kernel timing tool behi
   python bench_kernel.py eltwise    ROWS D DTYPE [REPS]         (out = a + b[broadcast row])
   python bench_kernel.py nchw2nhwc  N C H W DTYPE [REPS]        (input re-layout with channel padding and halo)
   python bench_kernel.py push       BYTES NDST [REPS]           (the gather's multi-destination copy, destinations on this GPU)
-PREC: bf16 | tf32 | tf32x3 | fp32      DTYPE: bf16 | f32
+  python bench_kernel.py rotary     TOKENS HEADS D DTYPE [REPS]
+  python bench_kernel.py kvappend   BATCH NEW HEADS KV_HEADS D PAGE DTYPE [REPS]     (keys and queries turned, one axis)
+  python bench_kernel.py paged      BATCH NEW KEYS HEADS KV_HEADS D PAGE DTYPE [REPS] [WINDOW SINKS]
+PREC: bf16 | tf32 | tf32x3 | fp32      DTYPE: bf16 | f32 (rotary, kvappend and paged: f16 too)
 Every repetition is timed with CUDA events on the launching stream after an L2 flush (a 256 MB write); the line
 printed is the median: `<kind> ... ms <t> TFLOP/s <x> GB/s <y> status <word>` with the algorithmic FLOPs and bytes.
 """
@@ -53,7 +56,15 @@ def report(label, ms, flops, nbytes):
 
 
 def _dt(name):
-    return torch.bfloat16 if name in ("bf16", "bfloat16") else torch.float32
+    return torch.bfloat16 if name in ("bf16", "bfloat16") else torch.float16 if name in ("f16", "float16") else torch.float32
+
+
+def _paged_batch(batch, new, keys, kv_heads, d, page, dt):
+    """Caches with pages in random order, page table, row starts and lengths of `batch` equal sequences."""
+    per = -(-keys // page)
+    k, v = (torch.randn(batch * per, page, kv_heads, d, device="cuda", dtype=dt) for _ in range(2))
+    table = torch.randperm(batch * per, device="cuda").to(torch.int32).view(batch, per)
+    return k, v, table, torch.arange(batch + 1, device="cuda", dtype=torch.int32) * new, torch.full((batch,), keys, device="cuda", dtype=torch.int32)
 
 
 def main(argv):
@@ -158,6 +169,38 @@ def main(argv):
         ms = timed(lambda: C.check(C.lib().llc_cuda_push_rows(src.data_ptr(), ptrs, ndst, 0, nbytes, st)), reps)
         assert all(torch.equal(d, src) for d in dsts)
         report(" ".join(argv), ms, 0.0, (1 + ndst) * nbytes)
+    elif kind == "rotary":
+        from llcompiler_b200.executor import rotary
+        tokens, heads, d = (int(a) for a in argv[1:4])
+        dt = _dt(argv[4]); reps = int(argv[5]) if len(argv) > 5 else 7
+        x = torch.randn(tokens, heads, d, device="cuda").to(dt)
+        out, pos = torch.empty_like(x), torch.arange(tokens, device="cuda")
+        freq = 10000.0 ** (-torch.arange(d // 2, device="cuda", dtype=torch.float64) / (d // 2))
+        ms = timed(lambda: rotary(x, pos, freq, out=out), reps)
+        report(" ".join(argv), ms, 3.0 * x.numel(), 2 * x.numel() * x.element_size() + 8 * tokens)
+    elif kind == "kvappend":
+        from llcompiler_b200.executor import kv_append
+        batch, new, heads, kv_heads, d, page = (int(a) for a in argv[1:7])
+        dt = _dt(argv[7]); reps = int(argv[8]) if len(argv) > 8 else 7
+        caches = _paged_batch(batch, new, new + 1000, kv_heads, d, page, dt)
+        qkv = torch.randn(batch * new, heads + 2 * kv_heads, d, device="cuda").to(dt)
+        q, k, v = qkv[:, :heads], qkv[:, heads : heads + kv_heads], qkv[:, heads + kv_heads :]
+        out = torch.empty(batch * new, heads, d, device="cuda", dtype=dt)
+        freq = 10000.0 ** (-torch.arange(d // 2, device="cuda", dtype=torch.float64) / (d // 2))
+        ms = timed(lambda: kv_append(k, v, *caches, q=q, inv_freq=freq, q_out=out), reps)
+        report(" ".join(argv), ms, 3.0 * batch * new * (heads + kv_heads) * d, 2 * qkv.numel() * qkv.element_size())
+    elif kind == "paged":
+        from llcompiler_b200.executor import paged_attention
+        batch, new, keys, heads, kv_heads, d, page = (int(a) for a in argv[1:8])
+        dt = _dt(argv[8]); reps = int(argv[9]) if len(argv) > 9 else 7
+        window, sinks = (int(argv[10]), int(argv[11])) if len(argv) > 11 else (0, 0)
+        caches = _paged_batch(batch, new, keys, kv_heads, d, page, dt)
+        q = torch.randn(batch * new, heads, d, device="cuda").to(dt)
+        out = torch.empty_like(q)
+        ms = timed(lambda: paged_attention(q, *caches, window=window, sinks=sinks, max_q=new, out=out), reps)
+        seen = [min(p + 1, window + min(sinks, max(0, p + 1 - window))) if window else p + 1 for p in range(keys - new, keys)]
+        read = keys if not window else min(keys, window + new - 1 + sinks)
+        report(" ".join(argv), ms, 4.0 * batch * sum(seen) * heads * d, (2 * q.numel() + 2 * batch * read * kv_heads * d) * q.element_size())
     else:
         raise SystemExit(__doc__)
     torch.cuda.synchronize()

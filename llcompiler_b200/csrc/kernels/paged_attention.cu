@@ -114,6 +114,11 @@ int checkAndFill(const LlcPagedAttentionParams* p, PagedArgs* a) {
   a->table = p->page_table; a->qStart = p->q_start; a->kvLen = p->kv_len; a->badPages = p->bad_pages;
   a->qSt = p->q_st; a->qSh = p->q_sh; a->oSt = p->o_st; a->oSh = p->o_sh;
   a->kcSp = p->kc_sp; a->kcSn = p->kc_sn; a->kcSh = p->kc_sh; a->vcSp = p->vc_sp; a->vcSn = p->vc_sn; a->vcSh = p->vc_sh;
+  // the stride of a dim of one element says nothing: one that fits every kernel
+  if (p->tokens == 1) a->qSt = a->oSt = 0;
+  if (p->heads == 1) a->qSh = a->oSh = 0;
+  if (p->kv_heads == 1) a->kcSh = a->vcSh = (p->d + 7) / 8 * 8;
+  if (p->num_pages == 1) a->kcSp = a->vcSp = (p->d + 7) / 8 * 8;
   a->tableS0 = p->table_s0; a->tokens = p->tokens; a->numPages = p->num_pages; a->pageSize = p->page_size;
   a->reach = (int)(p->table_width * p->page_size);
   a->maxQ = p->max_q < p->tokens ? p->max_q : p->tokens;
@@ -142,7 +147,8 @@ int decodeRows(const PagedArgs& a) {
   if (rows <= 32) return rows <= 16 ? 16 : 32;
   // few sequences of few keys fit beside the chunks' tiles, and a launch less is worth more (nine sequences of up to 2048 keys, one of them
   // a single token: 35 us with one kernel, 47 with both)
-  if (a.batch == 1 || (a.reach <= 4096 && a.batch * a.kvHeads <= deviceSMs())) return 0;
+  const long long seen = (long long)a.window + a.sinks < a.reach ? (long long)a.window + a.sinks : a.reach;   // keys that a token can see
+  if (a.batch == 1 || (seen <= 4096 && a.batch * a.kvHeads <= deviceSMs())) return 0;
   return a.group <= 16 ? 16 : a.group <= 32 ? 32 : 0;
 }
 

@@ -246,14 +246,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += x; }
     if (lane == 31) sScan[warp] = run;
-    if (threadIdx.x == 0) {
-      plan->seq = -1;
-      for (int i = 0; i < C::kSlots; ++i) { mbarInit(&kvFull[i], 1); mbarInit(&kvEmpty[i], 1); }
-      for (int t = 0; t < 2; ++t) { mbarInit(&sFull[t], 1); mbarInit(&pReady[t], kSoftmaxWarps / 2); mbarInit(&oFull[t], 1); }
-      mbarInit(qReady, kSoftmaxWarps);
-      *abortWord = 0;
+    if (warp == kLoaderWarp) {                        // not the warp that will work out the plan of a lone sequence
+      if (lane == 0) { plan->seq = -1; *abortWord = 0; prefetchTensorMap(&mapK); prefetchTensorMap(&mapV); }
+      const int per = 2 * C::kSlots;                  // then sFull, pReady, oFull of two tiles, qReady
+      if (lane < per + 7) mbarInit(&kvFull[lane], lane == per + 2 || lane == per + 3 ? kSoftmaxWarps / 2 : lane == per + 6 ? kSoftmaxWarps : 1);
       fenceBarrierInit();
     }
+    static_assert(2 * C::kSlots + 7 <= 32, "a lane a barrier");
     __syncthreads();
     int before = run - mine, all = 0;
 #pragma unroll
@@ -290,13 +289,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
       plan->pair = pair; plan->split = split; plan->splits = splits;
       if (splits > 1 && split == 0) a.records[1 + pair] = make_int4(i, want - before, 0, 0);
     }
+    if (warp == kIssuerWarp) tmemAlloc(tmemSlot, 512);
+    tcFenceBefore();
     __syncthreads();
+    tcFenceAfter();
   }
-  if (plan->seq < 0) return;                          // fewer tiles than the grid has room for
-  if (warp == kIssuerWarp) tmemAlloc(tmemSlot, 512);
-  tcFenceBefore();
-  __syncthreads();
-  tcFenceAfter();
+  if (plan->seq < 0) {                                // fewer tiles than the grid has room for
+    if (warp == kIssuerWarp) tmemDealloc(*tmemSlot, 512);
+    return;
+  }
   const uint32_t tmem = *tmemSlot;
 
   // Registers: 96 a thread at launch, 640 threads; 104 for the 512 softmax threads and 64 for the other 128 make the same sum.
@@ -304,7 +305,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == kLoaderWarp) {
       // ---------------------------------------------------------------- loader: items K, V, K, V, ...
-      if (lane == 0) { prefetchTensorMap(&mapK); prefetchTensorMap(&mapV); }
       const int boxes = kKeys / a.boxRows, loads = boxes * (D / 64), box = lane % boxes, half = lane / boxes;
       bool ok = true;
       uint32_t item = 0;
@@ -646,7 +646,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     pairBarrier(bar);
     if (!cut) {
       const long long oOff = (long long)(plan->qBegin + oTok) * p.oSt + oHead * p.oSh;
-#pragma unroll 4
+#pragma unroll
       for (int i = 0; i < 16; i += kRowsAtOnce) {
         const int src = side * 16 + i + lane / kChunks, c = lane % kChunks, rr = q4 * 32 + src;
         const long long off = __shfl_sync(0xffffffffu, oOff, src);

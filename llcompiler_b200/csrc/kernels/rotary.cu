@@ -312,8 +312,10 @@ extern "C" int llc_cuda_rotary(const LlcRotaryParams* p, void* stream) {
   a.qSt = p->x_st; a.qSh = p->x_sh; a.qoSt = p->o_st; a.qoSh = p->o_sh; a.posSa = p->pos_sa;
   a.tokens = p->tokens; a.nQ = (int)p->heads; a.d = (int)p->d; a.interleaved = p->interleaved != 0;
   const int64_t vec = 16 / dtypeBytes(p->dtype);
-  const bool al = aligned16(p->x) && aligned16(p->out) && p->d % vec == 0 && p->pairs % vec == 0 && p->x_st % vec == 0 && p->x_sh % vec == 0 &&
-                  p->o_st % vec == 0 && p->o_sh % vec == 0;
+  if (p->tokens == 1) a.qSt = a.qoSt = 0;              // the stride of a dim of one element says nothing
+  if (p->heads == 1) a.qSh = a.qoSh = 0;
+  const bool al = aligned16(p->x) && aligned16(p->out) && p->d % vec == 0 && p->pairs % vec == 0 && a.qSt % vec == 0 && a.qSh % vec == 0 &&
+                  a.qoSt % vec == 0 && a.qoSh % vec == 0;
   return chooseType<false>(a, p->dtype, al, (cudaStream_t)stream);
 }
 
@@ -344,7 +346,10 @@ extern "C" int llc_cuda_kv_append(const LlcKvAppendParams* p, void* stream) {
   const int64_t vec = 16 / dtypeBytes(p->dtype);
   bool al = p->d % vec == 0 && a.pairs % vec == 0;
   for (const void* x : {p->k, p->v, (const void*)p->k_cache, (const void*)p->v_cache}) al = al && aligned16(x);
-  if (nq) al = al && aligned16(p->q) && aligned16(p->q_out) && p->q_st % vec == 0 && p->q_sh % vec == 0 && p->qo_st % vec == 0 && p->qo_sh % vec == 0;
-  for (int64_t s : {p->k_st, p->k_sh, p->v_st, p->v_sh, p->kc_sp, p->kc_sn, p->kc_sh, p->vc_sp, p->vc_sn, p->vc_sh}) al = al && s % vec == 0;
+  if (p->tokens == 1) a.qSt = a.qoSt = a.kSt = a.vSt = 0;   // the stride of a dim of one element says nothing
+  if (nq <= 1) a.qSh = a.qoSh = 0;
+  if (p->kv_heads == 1) a.kSh = a.vSh = a.kcSh = a.vcSh = 0;
+  if (nq) al = al && aligned16(p->q) && aligned16(p->q_out);
+  for (long long s : {a.qSt, a.qSh, a.qoSt, a.qoSh, a.kSt, a.kSh, a.vSt, a.vSh, a.kcSp, a.kcSn, a.kcSh, a.vcSp, a.vcSn, a.vcSh}) al = al && s % vec == 0;
   return chooseType<true>(a, p->dtype, al, (cudaStream_t)stream);
 }
