@@ -7,8 +7,8 @@
 // compute 128 rows for the 4 to 16 that exist, with a longer chain from scores to values).
 // Work: the blocks of 16 keys of all (sequence, key head) pairs form one line, cut into equal shares, one a WARP: ragged batches and
 // single long sequences load every SM alike, and no warp waits for another.  A warp is its own producer: when a block has been
-// used, its lanes start the TMA loads of the block that comes a ring's length later (12 KB of 16 rows x 64 element boxes in flight for
-// every warp, eight warps an SM).  A pair that a share's end cuts leaves its parts' sums in the workspace, which a second kernel joins
+// used, its lanes start the TMA loads of the block that comes a ring's length later (boxes of 16 rows x 64 elements,
+// eight warps an SM).  A pair that a share's end cuts leaves its parts' sums in the workspace, which a second kernel joins
 // (launched early, it waits for this one on the device).  Few and short pairs (SPLIT false) take a CTA each instead, whose warps
 // take the blocks in turn and meet in shared memory: the second launch costs more than it saves there.
 // Before this, four warps shared blocks of 64 keys and met at the end of every pair: 10000 cycles from one pair to the next.
@@ -33,7 +33,9 @@ template <int D, int MT> struct Config {
   static constexpr int kBox = kKeys * 128;         // bytes of 16 keys x 64 elements
   static constexpr int kTensor = kBox * (D / 64);  // K or V of a block
   static constexpr int kBlock = 2 * kTensor;
-  static constexpr int kStages = 24 * 1024 / kBlock;
+  // 16 KB in flight for a warp, 128 KB for an SM; with 24 KB everything an SM asks for stands in a longer line (32 x 8192 keys of 8 heads
+  // of 128: 177 us, 189 with 24 KB; one sequence of 131072: 97 and 101)
+  static constexpr int kStages = 16 * 1024 / kBlock;
   static constexpr int kRing = kWarps * kStages * kBlock;
   static constexpr int kMisc = 512 + 2 * kWarps * kRows * 4;   // barriers and the shares' starts, then m and l of every warp's rows
   static constexpr int kSmem = kRing + kMisc;
@@ -228,9 +230,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
     load.unit += step;
     if (load.unit >= load.end) { loading = SPLIT && load.next(p, C::kRows); k = 32; }
   };
-#pragma unroll 1
-  for (int i = 0; i < C::kStages; ++i) issue();
-
   const uint32_t ringAddr = smemAddr(ring);
   const int g4 = lane >> 2, c4 = lane & 3;         // a thread's row (and row + 8) of a tile, its pair of columns
   // K: matrices (keys 0-7, d 0-7), (keys 0-7, d 8-15), (keys 8-15, d 0-7), (keys 8-15, d 8-15) of a 16 x 16 step
@@ -262,6 +261,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
           qf[mt][ks][2 + r] = row < rows ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8) : 0u;
         }
       }
+    // The first loads start behind the queries': what an SM asks for comes in about the order of asking.
+    if (loaded == 0)
+#pragma unroll 1
+      for (int i = 0; i < C::kStages; ++i) issue();
     float o[MT][D / 8][4], m[MT][2], l[MT][2];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
