@@ -172,6 +172,7 @@ extern "C" int llc_cuda_paged_attention(const LlcPagedAttentionParams* p, void* 
   if (a.tokens == 0 || a.batch == 0 || a.maxQ == 0) return LLC_OK;
   if (!p->q || !p->out || !p->q_start || !p->kv_len || (a.reach > 0 && !p->page_table) || (p->num_pages > 0 && (!p->k_cache || !p->v_cache)))
     return setError(LLC_ERR_ARGUMENT, "llc argument: paged_attention null operand");
+  if (reinterpret_cast<uintptr_t>(p->workspace) & 15) return setError(LLC_ERR_ARGUMENT, "llc argument: paged_attention workspace must be 16-byte aligned");
   const cudaStream_t st = (cudaStream_t)stream;
   if (!tensorTypes(a)) return pagedRows(a, st);
   const int few = decodeRows(a);

@@ -281,6 +281,32 @@ def test_one_long_sequence_among_many_short_ones():
     _check(out, q, k, v, table, q_start, kv_len)
 
 
+@pytest.mark.parametrize("batch", [127, 300, 700])
+def test_large_batches_of_few_tokens(batch):
+    """More sequences than a block has threads: single tokens, and the same with some chunks among them and sequences without any."""
+    kv_heads, d, page = 1, 64, 16
+    lens = [1 + (i * 13) % 40 for i in range(batch)]
+    k, v, table, q_start, kv_len = R.make_batch([1] * batch, lens, page, kv_heads, d, torch.float16, width=40)
+    q = _q(batch, 2, d, torch.float16)
+    _check(_run(q, k, v, table, q_start, kv_len, max_q=1), q, k, v, table, q_start, kv_len)
+    new = [(20 if i % 97 == 5 else (i * 7) % 3) for i in range(batch)]
+    lens = [n + (i * 13) % 40 for i, n in enumerate(new)]
+    k, v, table, q_start, kv_len = R.make_batch(new, lens, page, kv_heads, d, torch.float16, width=300)
+    q = _q(sum(new), 2, d, torch.float16)
+    _check(_run(q, k, v, table, q_start, kv_len, max_q=20), q, k, v, table, q_start, kv_len)
+
+
+def test_the_same_memory_for_queries_and_output():
+    for new, lens in (([1, 1, 1], [700, 40, 1300]), ([40, 1], [90, 60]), ([40], [5000])):
+        k, v, table, q_start, kv_len = R.make_batch(new, lens, 16, 1, 128, torch.bfloat16)
+        q = _q(sum(new), 2, 128, torch.bfloat16)
+        from llcompiler_b200.executor import paged_attention
+        dev = q.to(DEV)
+        got = paged_attention(dev, *(t.to(DEV) for t in (k, v, table, q_start, kv_len)), max_q=max(new), out=dev)
+        assert got is dev
+        _check(dev, q, k, v, table, q_start, kv_len)
+
+
 def test_other_streams():
     k, v, table, q_start, kv_len = R.make_batch([1] * 6, [900, 20, 450, 3, 1500, 64], 16, 2, 128, torch.bfloat16)
     q = _q(6, 8, 128, torch.bfloat16)

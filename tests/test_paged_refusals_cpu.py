@@ -62,6 +62,7 @@ def test_append_refuses(kw, code):
     (dict(tokens=-1), 3), (dict(batch=-1), 3), (dict(heads=0), 3), (dict(kv_heads=0), 3), (dict(heads=5), 3), (dict(d=0), 3), (dict(d=257), 2), (dict(max_q=-1), 3),
     (dict(window=-1), 3), (dict(sinks=-1), 3), (dict(page_size=0), 3), (dict(dtype=3), 2), (dict(q=None), 3), (dict(out=None), 3), (dict(k_cache=None), 3), (dict(v_cache=None), 3),
     (dict(page_table=None), 3), (dict(q_start=None), 3), (dict(kv_len=None), 3), (dict(page_size=1 << 20, table_width=1 << 20), 2), (dict(tokens=1 << 31), 2),
+    (dict(workspace=c_void_p((1 << 20) + 8), workspace_bytes=1 << 20), 3),
 ])
 def test_attention_refuses(kw, code):
     p = _attend(**kw)
