@@ -222,6 +222,7 @@ int llc_cuda_kv_append(const LlcKvAppendParams* p, void* stream);
  * A slot whose page number is outside [0, num_pages) reads as zeros (key and value) and each such page that a query sees is
  * counted in *bad_pages (at least once, or more often) when that is not NULL.  Nothing else of the cache is read into the
  * result: slots past kv_len, pages before the window and unused pages may hold anything.
+ * out may be q itself (same address, same strides).
  * max_q: at least the largest number of new tokens of a sequence; a sequence that has more is left out.
  * f32, bf16 and f16, all tensors alike, unit stride along d, d <= 256.  bf16 and f16 with d 64 or 128, page_size a power of
  * two >= 16, strides of 16 bytes' multiples and 16-byte aligned pointers run on the tensor cores, everything else

@@ -15,6 +15,8 @@ constexpr int kMaxD = 256;
 
 // One block per (token, head): the warps take the visible keys in turn, each with a running maximum and sum, lane l holding
 // elements l, l + 32, ... of the row, and meet in shared memory at the end.  out = sum_w o_w 2^(m_w - m) / sum_w l_w 2^(m_w - m).
+// Bound: the latency of a key at a time and the instructions of its dot product; every head of a group reads the keys anew.  16 sequences
+// of up to 4096 keys, 32 heads of 128 in bf16: 572 us, where the tensor-core kernels take 38; it is for what those do not take.
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedArgs p) {
   __shared__ float sM[kWarps], sL[kWarps], sO[kWarps][kMaxD];
