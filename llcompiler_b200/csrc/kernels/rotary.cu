@@ -6,7 +6,7 @@
 // 64-bit product, its whole part is dropped there, and only the fraction (at most half a turn) becomes a float.
 // Bound: memory; every element is read once and written once.  The sine and cosine of a (token, pair) are computed once per
 // block into shared memory and used by all heads of the token; the block's loads of x are under way meanwhile.  Measured, bf16: 20736 tokens
-// of 32 heads of 128 55 us (6.1 TB/s), 15286 tokens of 32 + 2 x 8 heads into a cache 74 us (5.1 TB/s).
+// of 32 heads of 128 55 us (6.1 TB/s), 15285 tokens of 32 + 2 x 8 heads into a cache 74 us (5.1 TB/s).
 #include <cuda_fp16.h>
 
 #include "common.cuh"

@@ -71,11 +71,13 @@ def attention_tolerance(want, size, largest, dtype):
     """One rounding of the result at the store, one of each weight to the tensors' type before the second product: half a step
     (u) each, relative to the value and to the weighted sum of |v|.  A score is a sum of d products in 32 bits whose steps
     (2^-23, the tensor core cuts off) add up to at most d 2^-23 of sum |q k|; a score that is off by x scales its weight by
-    e^x, in the sum of weights as well: twice that.  The exponential and the sums of weights: 2^-18 for up to some hundred keys.
-    The weights are taken relative to a maximum that may lag by 2^8, which costs no accuracy."""
+    e^x, in the sum of weights as well: twice that.  A quarter of a chunk's exponentials are polynomials whose relative error
+    is at most 2^-13.7 (bf16; f32 has none of them) or 2^-18.5 (f16), again in the sum as well: 2^-12.7 and 2^-17.5; the
+    hardware's exponential and the sums of weights add 2^-18 for up to some thousand keys.  The weights are taken
+    relative to a maximum that may lag by 2^8, which costs no accuracy."""
     u = torch.finfo(dtype).eps / 2
     d = want.shape[-1]
-    return want.abs() * u * (1 + 2.0 ** -7) + size * (u + 2 * largest * d * 2.0 ** -23 + 2.0 ** -18) + 1e-30 + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    return want.abs() * u * (1 + 2.0 ** -7) + size * (u + 2 * largest * d * 2.0 ** -23 + (2.0 ** -12.7 if dtype == torch.bfloat16 else 2.0 ** -17.5) + 2.0 ** -18) + 1e-30 + (2.0 ** -25 if dtype == torch.float16 else 0.0)
 
 
 def make_batch(new, lens, page, kv_heads, d, dtype, seed=0, heads_first=False, spare=2, width=None, fill=None):
