@@ -6,7 +6,7 @@
 // 64-bit product, its whole part is dropped there, and only the fraction (at most half a turn) becomes a float.
 // Bound: memory; every element is read once and written once.  The sine and cosine of a (token, pair) are computed once per
 // block into shared memory and used by all heads of the token; the block's loads of x are under way meanwhile.  Measured, bf16: 20736 tokens
-// of 32 heads of 128 55 us (6.1 TB/s), 15285 tokens of 32 + 2 x 8 heads into a cache 74 us (5.1 TB/s).
+// of 32 heads of 128 55 us (6.1 TB/s), 15285 tokens of 32 + 2 x 8 heads into a cache 70 us (5.4 TB/s).
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -248,12 +248,13 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotArgs p) {
 template <typename T, int VEC, bool CACHE>
 int launch(RotArgs& a, cudaStream_t st) {
   constexpr int kUnroll = unrolled<CACHE>();
-  // Tokens of a block: a power of two, as many as give every thread kUnroll rows, fewer while the grid has less than two blocks an SM,
+  // Tokens of a block: a power of two, as many as give every thread kUnroll rows (twice that when it writes a cache, whose lookups are
+  // then shared by more rows: 70 us against 73.5 for 15285 tokens), fewer while the grid has less than two blocks an SM,
   // and no more than shared memory has room for (48 KB without an opt-in).
   a.rows = CACHE ? a.nQ + 2 * a.nK : a.nQ;
   a.perRow = (a.d + 2 * VEC - 1) / (2 * VEC);
   int tok = 1;
-  while (2 * tok <= kMaxTokens && 2LL * tok * a.rows * a.perRow <= kThreads * kUnroll && 2LL * tok * a.perRow <= kThreads && 2LL * tok * a.pairs * (long long)sizeof(float2) <= 40960 &&
+  while (2 * tok <= kMaxTokens && 2LL * tok * a.rows * a.perRow <= kThreads * kUnroll * (CACHE ? 2 : 1) && 2LL * tok * a.perRow <= kThreads && 2LL * tok * a.pairs * (long long)sizeof(float2) <= 40960 &&
          a.tokens >= 2LL * tok * 2 * deviceSMs())
     tok *= 2;
   a.tokensPerBlock = tok;
