@@ -168,6 +168,38 @@ def test_lengths_and_rows_out_of_range_stay_inside():
     assert torch.isfinite(out.float()).all()
 
 
+def test_empty_batches_pools_and_tables():
+    from llcompiler_b200.executor import kv_append, paged_attention, rotary
+    bf = dict(device=DEV, dtype=torch.bfloat16)
+    i32 = lambda *v: torch.tensor(v, device=DEV, dtype=torch.int32)
+    pool, none = torch.zeros(3, 16, 2, 64, **bf), torch.zeros(0, 16, 2, 64, **bf)
+    q, k = torch.ones(3, 4, 64, **bf), torch.ones(3, 2, 64, **bf)
+    # no tokens
+    assert rotary(q[:0], torch.zeros(0, device=DEV, dtype=torch.int64), R.inv_freq(32).to(DEV)).shape == (0, 4, 64)
+    assert paged_attention(q[:0], pool, pool, i32(0)[None], i32(0, 0), i32(5)).shape == (0, 4, 64)
+    # no sequences: nobody's rows
+    out = torch.full_like(q, 5.0)
+    table = torch.zeros(0, 4, device=DEV, dtype=torch.int32)
+    paged_attention(q, pool, pool, table, i32(0), i32(), out=out)
+    kv_append(k, k, pool, pool, table, i32(0), i32(), q=q, q_out=out)
+    assert (out == 5).all() and (pool == 0).all()
+    # a pool without pages: every page is a bad one and reads as zeros; a table without columns: nothing is visible
+    bad = i32(0)
+    assert (paged_attention(q, none, none, i32(0, 0)[None], i32(0, 3), i32(3), max_q=3, bad_pages=bad) == 0).all() and int(bad) >= 1
+    assert (paged_attention(q, pool, pool, torch.zeros(1, 0, device=DEV, dtype=torch.int32), i32(0, 3), i32(3), max_q=3) == 0).all()
+    bad.zero_()
+    kv_append(k, k, none, none, i32(0, 0)[None], i32(0, 3), i32(3), bad_pages=bad)
+    kv_append(k, k, pool, pool, torch.zeros(1, 0, device=DEV, dtype=torch.int32), i32(0, 3), i32(3), bad_pages=bad)
+    assert int(bad) == 6 and (pool == 0).all()
+    # rows before the first sequence are nobody's either
+    out.fill_(5.0)
+    kv_append(k, k, pool, pool, i32(1)[None], i32(2, 3), i32(1), q=q, q_out=out)
+    assert (out[:2] == 5).all() and (out[2] == 1).all() and (pool[1, 0] == 1).all() and int(pool.sum()) == 128
+    out.fill_(5.0)
+    paged_attention(q, pool, pool, i32(1)[None], i32(2, 3), i32(1), max_q=1, out=out)
+    assert (out[:2] == 5).all() and (out[2] == 1).all()
+
+
 def test_strided_queries_and_output():
     k, v, table, q_start, kv_len = R.make_batch([3, 40], [30, 90], 16, 2, 64, torch.float16)
     qkv = _q(43, 4 + 2 + 2, 64, torch.float16)
