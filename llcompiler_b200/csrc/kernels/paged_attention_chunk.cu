@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const ChunkArgs a
     const float m = part[(long long)i * C::kPart + kTileRows * D + r], l = part[(long long)i * C::kPart + kTileRows * (D + 1) + r];
     const float f = m == -INFINITY ? 0.f : exp2Fast(m - top);
     if (side == 0) sF[i][r] = f;
-    if (m != -INFINITY) sum += l * f;
+    sum += l * f;                                     // a part without a maximum weighs nothing, unless its scores are NaN: then l is
   }
   __syncthreads();
   if (row >= rows) return;
@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const ChunkArgs a
 #pragma unroll 4
     for (int i = 0; i < splits; ++i) {
       const float f = sF[i][r];
-      if (f != 0.f) {                                 // a part that saw nothing may hold anything
+      if (f != 0.f) {
         const float4 v = *reinterpret_cast<const float4*>(part + (long long)i * C::kPart + ((long long)c * kTileRows + r) * 4);
         x.x = fmaf(v.x, f, x.x); x.y = fmaf(v.y, f, x.y); x.z = fmaf(v.z, f, x.z); x.w = fmaf(v.w, f, x.w);
       }

@@ -1,0 +1,73 @@
+"""Attention over the paged cache where rows, values or tables are not ordinary: NaN and infinite rows, tables much wider than the sequences,
+wide groups, captured chunks."""
+import pytest
+import torch
+
+import paged_reference as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _q(tokens, heads, d, dtype, seed=9):
+    return torch.randn(tokens, heads, d, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def _run(q, k, v, table, q_start, kv_len, window=0, sinks=0, **kw):
+    from llcompiler_b200.executor import paged_attention
+    dev = [R.to_device(t, DEV) for t in (q, k, v)]
+    return paged_attention(*dev, table.to(DEV), q_start.to(DEV), kv_len.to(DEV), window=window, sinks=sinks, **kw)
+
+
+def _owned(q_start, tokens):
+    t = torch.arange(tokens)
+    return (t >= int(q_start[0])) & (t < int(q_start[-1]))
+
+
+# the forms of the call: new tokens, lengths, heads, kv heads, d, page, type
+FORMS = {
+    "chunk": ([40, 33], [300, 90], 2, 1, 128, 64, torch.bfloat16),
+    "chunk_whole_blocks": ([200], [700], 4, 1, 64, 16, torch.float16),
+    "chunk_cut": ([40], [5000], 2, 1, 128, 64, torch.bfloat16),
+    "chunk_cut_d64": ([70, 66], [4000, 4200], 2, 2, 64, 32, torch.float16),
+    "decode": ([1, 1, 1], [77, 200, 16], 8, 2, 128, 16, torch.bfloat16),
+    "decode_cut": ([1, 2], [5000, 700], 4, 1, 64, 64, torch.float16),
+    "decode_cut_long": ([3], [40000], 4, 1, 128, 64, torch.bfloat16),
+    "plain_f32": ([3, 1], [50, 40], 4, 2, 64, 16, torch.float32),
+    "plain_d80": ([3, 1], [50, 40], 4, 2, 80, 16, torch.bfloat16),
+}
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_a_nan_query_is_nan_in_its_own_rows_only(form):
+    new, lens, heads, kv_heads, d, page, dtype = FORMS[form]
+    k, v, table, q_start, kv_len = R.make_batch(new, lens, page, kv_heads, d, dtype)
+    q = _q(sum(new) + 1, heads, d, dtype)
+    clean = _run(q, k, v, table, q_start, kv_len, max_q=max(new))
+    row = int(q_start[len(new) // 2])
+    q2 = q.clone()
+    q2[row, heads - 1] = float("nan")
+    got = _run(q2, k, v, table, q_start, kv_len, max_q=max(new))
+    assert got[row, heads - 1].isnan().all()
+    rest = _owned(q_start, len(q))[:, None].expand(-1, heads).clone()
+    rest[row, heads - 1] = False
+    assert torch.equal(got.cpu()[rest], clean.cpu()[rest]) and torch.isfinite(clean.cpu()[rest].float()).all()
+
+
+@pytest.mark.parametrize("form", ["chunk_cut", "chunk_cut_d64", "decode_cut"])
+@pytest.mark.parametrize("first", [True, False])
+def test_a_part_of_the_keys_that_is_nan_makes_its_rows_nan(form, first):
+    """Scores that are NaN from the first key on, up to every block's end (one of them is where the first part ends), or in the last keys
+    before the new tokens."""
+    from llcompiler_b200.executor import paged_attention
+    new, lens, heads, kv_heads, d, page, dtype = FORMS[form]
+    k, v, table, q_start, kv_len = R.make_batch(new, lens, page, kv_heads, d, dtype)
+    dev = [R.to_device(t, DEV) for t in (_q(sum(new), heads, d, dtype), k, v, table, q_start, kv_len)]
+    step = 128 if "chunk" in form else 16
+    last = (lens[0] - new[0]) // step
+    for i in range(last):
+        for j in range(i * step, (i + 1) * step) if first else range((last - 1 - i) * step, (last - i) * step):
+            if j % page == 0 or j % step == 0:
+                dev[1][int(table[0, j // page]), j % page : min(page, j % page + step)] = float("nan")
+        got = paged_attention(*dev, max_q=max(new))
+        assert got[: new[0]].isnan().all() and torch.isfinite(got[new[0] :].float()).all(), i
