@@ -218,7 +218,8 @@ int llc_cuda_kv_append(const LlcKvAppendParams* p, void* stream);
 /* out[t,h,:] = sum_j w_j v_j, w = softmax over the visible j of scale * q[t,h,:] . k_j, for the new tokens t of a ragged
  * batch over a paged cache that holds their keys and values already (llc_cuda_kv_append); query head h reads key head
  * h / (heads / kv_heads).  A token at place p sees the keys j <= p; with window > 0 only those with p - j < window, and the
- * first `sinks` keys of the sequence besides.  A token that sees nothing (kv_len smaller than its place asks for) gets zeros.
+ * first `sinks` keys of the sequence besides.  A token that sees nothing (kv_len smaller than its place asks for) gets zeros; one
+ * whose visible scores are all -inf gets NaN, which is what softmax makes of them.
  * A slot whose page number is outside [0, num_pages) reads as zeros (key and value) and each such page that a query sees is
  * counted in *bad_pages (at least once, or more often) when that is not NULL.  Nothing else of the cache is read into the
  * result: slots past kv_len, pages before the window and unused pages may hold anything.

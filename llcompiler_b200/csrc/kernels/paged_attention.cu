@@ -82,11 +82,12 @@ __global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedArgs
   float sum = 0.f, f[kWarps];
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) { f[w] = exp2f(sM[w] - base); sum += sL[w] * f[w]; }
+  const float divisor = divisorOf(sum, top, pos >= 0);
   for (int e = threadIdx.x; e < p.d; e += kWarps * 32) {
     float x = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) x += sO[w][e] * f[w];
-    storeAs(p.out, t * p.oSt + h * p.oSh + e, p.dtype, sum == 0.f ? 0.f : x / sum);
+    storeAs(p.out, t * p.oSt + h * p.oSh + e, p.dtype, x / divisor);
   }
 }
 

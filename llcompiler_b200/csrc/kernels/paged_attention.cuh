@@ -38,6 +38,11 @@ __device__ __forceinline__ long long pageOf(const PagedArgs& p, int b, long long
   return page >= 0 && page < p.numPages ? page : -1;
 }
 
+// What a row's sums are divided by.  A token at place 0 or later sees at least the key at its own place; one before place 0 sees none and gets
+// zeros.  `top` is the maximum of its scores: -inf where all that it sees score -inf, and then the softmax is 0 / 0, whatever the weights were taken
+// to be relative to a stand-in for that maximum.
+__device__ __forceinline__ float divisorOf(float sum, float top, bool sees) { return !sees ? INFINITY : top == -INFINITY ? NAN : sum; }
+
 // The keys that tokens at places first .. last of a sequence see, some of them at least: [0, sinkEnd) and [lo, hi).  Places below 0
 // (more new tokens than the length says) see nothing; they are clipped to -1, so that all of this fits 32 bits.
 struct Seen { int sinkEnd, lo, hi; };

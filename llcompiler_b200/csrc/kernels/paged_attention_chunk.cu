@@ -589,7 +589,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     const float base = m == -INFINITY ? 0.f : m - kShift;
     const bool cut = plan->splits > 1;
     float* part = a.parts + (((long long)plan->pair * 2 + t) * plan->splits + plan->split) * C::kPart;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = 1.f / divisorOf(l, m, pos >= 0);
     bool odd = false;
     if (cut && side == 0) {
       part[kTileRows * D + r] = m;
@@ -687,8 +687,8 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const ChunkArgs a
   }
   __syncthreads();
   if (row >= rows) return;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const long long tok = row / p.group;
+  const float inv = 1.f / divisorOf(sum, top, s.len - s.n + tok >= 0);
   const int head = (int)(pair % p.kvHeads) * p.group + (int)(row - tok * p.group);
   T* out = reinterpret_cast<T*>(p.out) + (s.begin + tok) * p.oSt + head * p.oSh;
   for (int c = side; c < D / 4; c += 2) {

@@ -395,7 +395,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
           if (row >= rows) continue;
           if (whole) {
             const int tok = row / p.group;
-            const float inv = l[mt][r] == 0.f ? 0.f : 1.f / l[mt][r];
+            const float inv = 1.f / divisorOf(l[mt][r], m[mt][r], pos[mt][r] >= 0);
             T* dst = reinterpret_cast<T*>(p.out) + (s.begin + tok) * p.oSt + (use.h * p.group + row - tok * p.group) * p.oSh + c4 * 2;
 #pragma unroll
             for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint32_t*>(dst + 8 * i) = pack2<T>(o[mt][i][2 * r] * inv, o[mt][i][2 * r + 1] * inv);
@@ -451,7 +451,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
           }
         }
         const int tok = row / p.group;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float inv = 1.f / divisorOf(sum, top, (long long)s.len - s.n + tok >= 0);
         T* dst = reinterpret_cast<T*>(p.out) + (s.begin + tok) * p.oSt + (use.h * p.group + row - tok * p.group) * p.oSh + at;
         uint32_t w[kEach / 2];
 #pragma unroll
@@ -508,13 +508,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
     const int tok = row / p.group;
     return reinterpret_cast<T*>(p.out) + (s.begin + tok) * p.oSt + (h * p.group + row - tok * p.group) * p.oSh;
   };
+  auto sees = [&](int row) { return (long long)s.len - s.n + row / p.group >= 0; };
   if (a.joinRows > 1 && parts <= 32) {
     const int row = row0 + warp;
     if (row >= rows) return;
     const float* part = a.slots + ((long long)pair + rec.x) * stride + row * (D + kTail);
     float2 ml = make_float2(-INFINITY, 0.f);
     if (lane < parts) ml = *reinterpret_cast<const float2*>(part + lane * stride + D);
-    const float top = warpMax(ml.x), f = ml.x == -INFINITY ? 0.f : exp2Fast(ml.x - top), total = warpSum(ml.y * f), inv = total == 0.f ? 0.f : 1.f / total;
+    const float top = warpMax(ml.x), f = ml.x == -INFINITY ? 0.f : exp2Fast(ml.x - top), total = warpSum(ml.y * f), inv = 1.f / divisorOf(total, top, sees(row));
     float x[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) x[e] = 0.f;
@@ -553,7 +554,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
       float y = 0.f, total = 0.f;
 #pragma unroll
       for (int w = 0; w < kJoinWarps; ++w) { y += sO[w][threadIdx.x]; total += sSum[w]; }
-      y = total == 0.f ? 0.f : y / total;
+      y /= divisorOf(total, top, sees(row));
       if constexpr (std::is_same<T, __half>::value) place(row)[threadIdx.x] = __float2half_rn(y);
       else place(row)[threadIdx.x] = __float2bfloat16_rn(y);
     }

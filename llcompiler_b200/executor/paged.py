@@ -75,8 +75,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     first ``sinks`` of the sequence.  Query head h reads key head ``h // (heads // kv_heads)``.  ``scale`` defaults to
     ``1 / sqrt(head_dim)``.  ``max_q`` bounds the new tokens of one sequence (default: all of them); a decoding step says 1,
     which lets the call choose the kernel for few rows; a sequence that has more is left out.  A token that sees nothing gets
-    zeros; rows of no sequence are not written.  Pages that are none of the pool's read as zeros and are counted in
-    ``bad_pages`` (one int32) if that is given."""
+    zeros, one whose visible scores are all -inf NaN (0 / 0); rows of no sequence are not written.  Pages that are none of the pool's
+    read as zeros and are counted in ``bad_pages`` (one int32) if that is given."""
     if isinstance(q, torch.Tensor) and q.is_cuda and q.get_device() == _current():
         return _ops.paged_attention(q, k_cache, v_cache, page_table, q_start, kv_len, scale, window, sinks, max_q, out, bad_pages)
     return _elsewhere(_ops.paged_attention, q, k_cache, v_cache, page_table, q_start, kv_len, scale, window, sinks, max_q, out, bad_pages)

@@ -71,3 +71,36 @@ def test_a_part_of_the_keys_that_is_nan_makes_its_rows_nan(form, first):
                 dev[1][int(table[0, j // page]), j % page : min(page, j % page + step)] = float("nan")
         got = paged_attention(*dev, max_q=max(new))
         assert got[: new[0]].isnan().all() and torch.isfinite(got[new[0] :].float()).all(), i
+
+
+def _against_definition(got, q, k, v, table, q_start, kv_len, window=0, sinks=0, scale=None):
+    """NaN where the definition has NaN, infinities where it has them, the rest within the tolerance (scores of infinite size are exact:
+    they weigh nothing)."""
+    scale = R.scale_of(q.shape[2]) if scale is None else scale
+    want, size, _ = R.attention(q, k, v, table, q_start, kv_len, scale, window, sinks)
+    finite_k, finite_v = (torch.where(torch.isfinite(t), t, torch.zeros((), dtype=t.dtype)) for t in (k, v))
+    _, _, largest = R.attention(q, finite_k, finite_v, table, q_start, kv_len, scale, window, sinks)
+    owned, got = _owned(q_start, len(q)), got.double().cpu()
+    want, got = want[owned], got[owned]
+    assert torch.equal(want.isnan(), got.isnan()), "NaN elsewhere"
+    ends = want.isinf()
+    assert torch.equal(want[ends], got[ends])
+    f = torch.isfinite(want)
+    tol = R.attention_tolerance(want, size[owned], largest, q.dtype)
+    assert ((got - want).abs() <= tol)[f].all(), float(((got - want).abs() / tol)[f].max())
+
+
+@pytest.mark.parametrize("form", [f for f in FORMS if f != "decode_cut_long"])   # the definition is slow to restate over so many keys
+@pytest.mark.parametrize("window", [0, 9])
+def test_rows_that_see_only_minus_infinity_are_nan_and_rows_that_see_nothing_zero(form, window):
+    """softmax of -inf alone is 0 / 0, in every kernel; a token without a visible key has zeros."""
+    new, lens, heads, kv_heads, d, page, dtype = FORMS[form]
+    for hide in ("all", "some", "few"):
+        k, v, table, q_start, kv_len = R.make_batch(new, lens, page, kv_heads, d, dtype)
+        q = _q(sum(new), heads, d, dtype).abs()               # positive: the product with a key of -inf is -inf
+        for j in range(lens[0] if hide == "all" else lens[0] - (new[0] + 1) // 2 if hide == "some" else 20):
+            k[int(table[0, j // page]), j % page] = float("-inf")
+        if hide == "few" and len(new) > 1:
+            kv_len[1] = new[1] // 2                           # the first of sequence 1's tokens see nothing
+        got = _run(q, k, v, table, q_start, kv_len, window, max_q=max(new))
+        _against_definition(got, q, k, v, table, q_start, kv_len, window)
