@@ -28,7 +28,9 @@ using namespace tc;
 constexpr int kSoftmaxWarps = 16, kLoaderWarp = 16, kIssuerWarp = 17;
 constexpr int kThreads = 20 * 32;          // the last two warps are idle: they fill the warpgroup that gives registers away
 constexpr int kTileRows = 128, kCtaRows = 256, kKeys = 128;
-constexpr int kCutBlocks = 12;            // least blocks of a part (nine sequences of up to 2048 keys: 59 us with 2, 35 with 12)
+// Least blocks of a part.  Nine sequences of up to 2048 keys: 59 us with 2, 35 with 12; 40 tokens of 32 heads over 500 keys: 48 us in parts of one
+// block, 17 whole.
+constexpr int kCutBlocks = 12;
 constexpr int kMaxSplits = 32;
 
 template <int D> struct Config {
@@ -47,10 +49,10 @@ struct ChunkArgs {
   PagedArgs p;
   int doneRows;                // sequences of at most so many rows are the decode kernel's
   int pageShift, boxRows;
-  int maxCut, maxSplits;       // CTAs that cut keys may fill, one and a half times the SMs (0: no key is cut), most parts of a tile's keys
+  int maxCut, maxSplits;       // CTAs that cut keys may fill, one and a half times the SMs (0: no key is cut), most parts of a pair's keys
   float scaleAbs, signQ;       // the scale's size; its sign goes into Q, so that the largest product is the largest score
-  int4* records;               // [0]: pairs of tiles of the call, parts of each; then of each pair its sequence and tile
-  float* parts;                // [pairs][2][parts][kPart]
+  int4* records;               // [0]: pairs of tiles of the call, CTAs of each; then of each pair its sequence, its tile and the parts of its keys
+  float* parts;                // [pairs][2][CTAs of a pair][kPart]
 };
 
 // What a tile's rows see.
@@ -102,6 +104,7 @@ struct Plan {
   int begin, end;              // units of this CTA's part of the keys
   int seq, tile;               // sequence (-1: nothing to do) and pair of tiles
   int pair, split, splits;     // (pair of tiles, key head), which part of its keys of how many
+  int ctas;                    // of each pair of the call
   int n, len;                  // of the sequence
   int row0, rows, qBegin;      // rows (token, query head) of the sequence: the host keeps tokens x query heads below 2^31
 };
@@ -236,7 +239,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
 
   asm volatile("griddepcontrol.launch_dependents;");
   // Which sequence and tiles.  The pairs of tiles, heads of one pair side by side, are taken from the last, which sees the most keys of its
-  // sequence.  Where they leave SMs idle (known here, from the lengths), each is cut into parts of its keys.
+  // sequence.  Where they leave SMs idle (known here, from the lengths), each has several CTAs and is cut into as many parts of its keys, if they
+  // have kCutBlocks blocks each: a table's width says nothing of a sequence's length.  The other CTAs of a short pair leave.
   int h;
   {
     // a thread keeps its (last) sequence: with up to kThreads of them nothing is read twice
@@ -260,10 +264,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) { const int x = sScan[w]; if (w < warp) before += x; all += x; }
     const long long pairs = (long long)all * p.kvHeads;
-    int splits = 1;
-    if (pairs > 0 && 2 * pairs <= a.maxCut) splits = min((2 * a.maxCut / 3 + (int)pairs / 2) / (int)pairs, a.maxSplits);   // nearest to the SMs
-    if (a.maxCut && blockIdx.x == 0 && threadIdx.x == 0) a.records[0] = make_int4((int)min(pairs, 0x7fffffffLL), splits, 0, 0);
-    const int pair = blockIdx.x / (unsigned)splits, split = blockIdx.x - pair * splits, tile = pair / p.kvHeads;
+    int ctas = 1;
+    if (pairs > 0 && 2 * pairs <= a.maxCut) ctas = min((2 * a.maxCut / 3 + (int)pairs / 2) / (int)pairs, a.maxSplits);   // nearest to the SMs
+    if (a.maxCut && blockIdx.x == 0 && threadIdx.x == 0) a.records[0] = make_int4((int)min(pairs, 0x7fffffffLL), ctas, 0, 0);
+    const int pair = blockIdx.x / (unsigned)ctas, split = blockIdx.x - pair * ctas, tile = pair / p.kvHeads;
     h = pair - tile * p.kvHeads;
     const int want = all - 1 - tile;
     if (want >= before && want < before + mine) {
@@ -280,23 +284,24 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
       const Tile tile0 = tileOf(p, s, row0, rows), tile1 = tileOf(p, s, row0 + kTileRows, rows);
       plan->seen = seenBy(p, tile0.first, tile1.last >= 0 ? tile1.last : tile0.last);
       const Blocks bl = blocksOf(plan->seen, kKeys);
-      const int share = (bl.count + splits - 1) / splits, begin = share * split < bl.count ? share * split : bl.count;
+      const int splits = max(1, min(ctas, bl.count / kCutBlocks));
       plan->units[0] = unitsOf(p, tile0, bl);
       plan->units[1] = unitsOf(p, tile1, bl);
       plan->bl = bl;
-      plan->begin = begin;
-      plan->end = begin + share < bl.count ? begin + share : bl.count;
-      plan->seq = i; plan->tile = want - before; plan->n = s.n; plan->len = s.len;
+      // at most 2^24 blocks and kMaxSplits parts; the last, whose blocks have masks, is never the longest
+      plan->begin = (bl.count * split + splits - 1) / splits;
+      plan->end = (bl.count * (split + 1) + splits - 1) / splits;
+      plan->seq = split < splits ? i : -1; plan->tile = want - before; plan->n = s.n; plan->len = s.len;
       plan->row0 = row0; plan->rows = rows; plan->qBegin = (int)s.begin;
-      plan->pair = pair; plan->split = split; plan->splits = splits;
-      if (splits > 1 && split == 0) a.records[1 + pair] = make_int4(i, want - before, 0, 0);
+      plan->pair = pair; plan->split = split; plan->splits = splits; plan->ctas = ctas;
+      if (ctas > 1 && split == 0) a.records[1 + pair] = make_int4(i, want - before, splits, 0);
     }
     if (warp == kIssuerWarp) tmemAlloc(tmemSlot, 512);
     tcFenceBefore();
     __syncthreads();
     tcFenceAfter();
   }
-  if (plan->seq < 0) {                                // fewer tiles than the grid has room for
+  if (plan->seq < 0) {                                // fewer tiles, or parts of this one's keys, than the grid has room for
     if (warp == kIssuerWarp) tmemDealloc(*tmemSlot, 512);
     return;
   }
@@ -588,7 +593,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
     l += loadShared(otherAt);
     const float base = m == -INFINITY ? 0.f : m - kShift;
     const bool cut = plan->splits > 1;
-    float* part = a.parts + (((long long)plan->pair * 2 + t) * plan->splits + plan->split) * C::kPart;
+    float* part = a.parts + (((long long)plan->pair * 2 + t) * plan->ctas + plan->split) * C::kPart;
     const float inv = 1.f / divisorOf(l, m, pos >= 0);
     bool odd = false;
     if (cut && side == 0) {
@@ -670,13 +675,13 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const ChunkArgs a
   __shared__ float sF[kMaxSplits][kTileRows];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const PagedArgs& p = a.p;
-  const int4 call = a.records[0];
-  const int pair = blockIdx.x >> 1, t = blockIdx.x & 1, r = threadIdx.x & 127, side = threadIdx.x >> 7, splits = call.y;
-  if (splits < 2 || pair >= call.x) return;
-  const int4 rec = a.records[1 + pair];
+  const int pair = blockIdx.x >> 1, t = blockIdx.x & 1, r = threadIdx.x & 127, side = threadIdx.x >> 7;
+  const int4 call = a.records[0], rec = a.records[1 + pair];   // the second read before it is known to be one: the workspace holds it in any case
+  const int splits = rec.z;
+  if (call.y < 2 || pair >= call.x || splits < 2) return;      // no pair of the call, or not cut and written already
   const Sequence s = sequenceOf(p, rec.x);
   const long long rows = (long long)s.n * p.group, row = (long long)rec.y * kCtaRows + t * kTileRows + r;
-  const float* part = a.parts + ((long long)pair * 2 + t) * splits * C::kPart;
+  const float* part = a.parts + ((long long)pair * 2 + t) * call.y * C::kPart;
   float top = -INFINITY, sum = 0.f;
   for (int i = 0; i < splits; ++i) top = fmaxf(top, part[(long long)i * C::kPart + kTileRows * D + r]);
   for (int i = 0; i < splits; ++i) {
@@ -706,16 +711,19 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const ChunkArgs a
 }
 
 // CTAs of the grid (a bound on the pairs of tiles times key heads from what the host knows), and whether keys may be cut: where the rows that
-// the call names would fill less than three quarters of the SMs, and enough
-// blocks of keys are left to each part: a part costs a CTA's start and end and its sums' way through memory, what eight blocks cost.
+// the call names would fill less than three quarters of the SMs, and the table's reach or the window leaves room for two parts of
+// kCutBlocks blocks (the device knows whether the sequences have them): a part costs a CTA's start and end and its sums' way through
+// memory, what eight blocks cost.
 struct Launch { long long ctas; int maxCut, maxSplits; };
 Launch launchOf(const PagedArgs& p) {
   Launch l{};
-  const long long each = (p.maxQ * p.group + kCtaRows - 1) / kCtaRows, most = p.tokens * p.group / kCtaRows + p.batch, sms = deviceSMs();
-  l.ctas = (each * p.batch < most ? each * p.batch : most) * p.kvHeads;
-  long long longest = p.reach;
-  if ((long long)p.window + p.sinks + kCtaRows < longest) longest = (long long)p.window + p.sinks + kCtaRows;
-  const long long splits = longest / (kCutBlocks * kKeys);
+  const long long each = (p.maxQ * p.group + kCtaRows - 1) / kCtaRows, tiles = p.tokens * p.group / kCtaRows + p.batch, sms = deviceSMs();
+  l.ctas = (each * p.batch < tiles ? each * p.batch : tiles) * p.kvHeads;
+  // blocks that a pair's rows see, at most: the rows of a pair belong to at most kCtaRows tokens; windows and sinks begin and end inside blocks
+  long long most = ((long long)p.reach + kKeys - 1) / kKeys;
+  const long long seen = ((long long)p.sinks + kKeys - 1) / kKeys + ((long long)p.window + kCtaRows + kKeys - 1) / kKeys + 1;
+  if (seen < most) most = seen;
+  const long long splits = most / kCutBlocks;
   l.maxSplits = (int)(splits < kMaxSplits ? splits : kMaxSplits);
   if (l.maxSplits > 1 && 4 * (p.tokens * p.group / kCtaRows) * p.kvHeads <= 3 * sms) l.maxCut = (int)(sms * 3 / 2);
   return l;

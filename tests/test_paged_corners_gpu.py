@@ -104,3 +104,17 @@ def test_rows_that_see_only_minus_infinity_are_nan_and_rows_that_see_nothing_zer
             kv_len[1] = new[1] // 2                           # the first of sequence 1's tokens see nothing
         got = _run(q, k, v, table, q_start, kv_len, window, max_q=max(new))
         _against_definition(got, q, k, v, table, q_start, kv_len, window)
+
+
+@pytest.mark.parametrize("new,lens,heads,kv_heads,d,page,dtype", [([40], [500], 2, 1, 128, 64, torch.float16), ([33, 70, 64], [900, 1535, 70], 2, 2, 64, 16, torch.float16),
+                                                                  ([40, 50], [5000, 300], 2, 1, 128, 64, torch.bfloat16), ([90], [1537], 1, 1, 64, 16, torch.float16)])
+def test_the_table_of_a_chunk_may_be_as_wide_as_a_server_likes(new, lens, heads, kv_heads, d, page, dtype):
+    """The keys are cut by the sequences' lengths: a table for 128 times the keys gives the same sums, bit for bit."""
+    k, v, table, q_start, kv_len = R.make_batch(new, lens, page, kv_heads, d, dtype)
+    q = _q(sum(new), heads, d, dtype)
+    tight = _run(q, k, v, table, q_start, kv_len, max_q=max(new))
+    wide = torch.full((len(new), 64 * table.shape[1]), -1, dtype=torch.int32)
+    wide[:, : table.shape[1]] = table
+    got = _run(q, k, v, wide, q_start, kv_len, max_q=max(new))
+    assert torch.equal(got, tight)
+    _against_definition(got, q, k, v, table, q_start, kv_len)
