@@ -180,30 +180,148 @@ __device__ __forceinline__ void storeShared(uint32_t at, float x) { asm volatile
 __device__ __forceinline__ float loadShared(uint32_t at) { float x; asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory"); return x; }
 __device__ __forceinline__ uint32_t bitsBelow(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
-// A row's sum over its visible keys among the blocks [begin, end) by multiply-adds, one warp a row: lane l gets elements l, l + 32, ...
-// Taken for a row whose sum came out NaN or infinite though its weights are finite: some value in the blocks is, and the products
-// multiply every value of a block by every row's weights, those that are 0 because the row does not see the value too.
-template <typename T, int D>
-__device__ __noinline__ void sumRow(const ChunkArgs& a, int b, int h, long long qOff, int pos, Blocks bl, int begin, int end, float base, float* o) {
+// A lane's elements of a row of D: kEach neighbours.
+template <int D> struct LaneOf { static constexpr int kEach = D / 32; using Pack = typename std::conditional<D == 128, uint2, uint32_t>::type; };
+template <typename T> __device__ __forceinline__ float2 twoFloats(uint32_t x);
+template <> __device__ __forceinline__ float2 twoFloats<__nv_bfloat16>(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
+template <> __device__ __forceinline__ float2 twoFloats<__half>(uint32_t x) { return __half22float2(*reinterpret_cast<__half2*>(&x)); }
+template <typename T, int D> __device__ __forceinline__ void unpack(const typename LaneOf<D>::Pack& x, float* f) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) { const float2 two = twoFloats<T>(w[i]); f[2 * i] = two.x; f[2 * i + 1] = two.y; }
+}
+__device__ __forceinline__ bool seesKey(const PagedArgs& p, int pos, int j) { return j <= pos && (pos - j < p.window || j < p.sinks); }
+
+// Values that are not finite, and the rows whose sums they spoil.  The products multiply every value of a block by every row's weight, the weights
+// that are 0 because the row does not see the key too, and 0 x NaN is NaN.  Only blocks that some row of the tile does not see whole have such
+// weights.  `Taint` holds, of each of a lane's columns, the last and the first such key (the sinks, which every later row sees, are not asked for
+// the first) and the first and last key with a NaN, over the blocks [begin, end) that the tile does not see whole.
+template <int D> struct Taint { int last[D / 32], first[D / 32], nan0[D / 32], nan1[D / 32]; };
+template <typename T, int D> __device__ __forceinline__ void findTaint(const ChunkArgs& a, const Plan* plan, int t, int h, Taint<D>& x) {
+  using L = LaneOf<D>;
   const PagedArgs& p = a.p;
   const int lane = threadIdx.x & 31;
-  float q[D / 32];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) { q[i] = (float)reinterpret_cast<const T*>(p.q)[qOff + lane + 32 * i] * a.signQ; o[i] = 0.f; }
-  for (int u = begin; u < end; ++u) {
-    const int j0 = keyOf(bl, u, kKeys);
+  for (int e = 0; e < L::kEach; ++e) { x.last[e] = x.nan0[e] = x.nan1[e] = -1; x.first[e] = 0x7fffffff; }
+  const Units n = plan->units[t];
+  const Seen seen = plan->seen;
+  for (int u = plan->begin; u < plan->end; ++u) {
+    if (!(u < n.sink || (u >= n.lo && u < n.hi)) || u < n.wholeSink || (u >= n.wholeLo && u < n.wholeHi)) continue;
+    const int j0 = keyOf(plan->bl, u, kKeys);
+#pragma unroll 8
     for (int j = j0; j < j0 + kKeys; ++j) {
-      if (!(j <= pos && (pos - j < p.window || j < p.sinks))) continue;
-      const long long page = pageOf(p, b, j >> a.pageShift), slot = j & ((1 << a.pageShift) - 1);
-      if (page < 0) continue;                         // its values are zeros
-      const T* k = reinterpret_cast<const T*>(p.k) + page * p.kcSp + slot * p.kcSn + h * p.kcSh;
-      const T* v = reinterpret_cast<const T*>(p.v) + page * p.vcSp + slot * p.vcSn + h * p.vcSh;
-      float dot = 0.f;
+      if (!(j < seen.sinkEnd || (j >= seen.lo && j < seen.hi))) continue;      // zeroed before the products
+      const long long page = pageOf(p, plan->seq, j >> a.pageShift);
+      if (page < 0) continue;
+      const T* v = reinterpret_cast<const T*>(p.v) + page * p.vcSp + (j & ((1 << a.pageShift) - 1)) * p.vcSn + h * p.vcSh;
+      float f[L::kEach];
+      unpack<T, D>(reinterpret_cast<const typename L::Pack*>(v)[lane], f);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) dot = fmaf((float)k[lane + 32 * i], q[i], dot);
-      const float w = exp2Fast(fmaf(warpSum(dot), a.scaleAbs, -base));
+      for (int e = 0; e < L::kEach; ++e) {
+        if (fabsf(f[e]) <= 3.402823466e38f) continue;
+        x.last[e] = j;                                // u and j only grow
+        if (j >= p.sinks && j < x.first[e]) x.first[e] = j;
+        if (f[e] != f[e]) { if (x.nan0[e] < 0) x.nan0[e] = j; x.nan1[e] = j; }
+      }
+    }
+  }
+}
+// Whether the sum of a row at `pos` may be spoilt: in some column a key that it does not see is not finite, and no NaN that it sees makes the column
+// NaN in any case.
+template <int D> __device__ __forceinline__ bool spoils(const PagedArgs& p, const Taint<D>& x, int pos) {
+  bool any = false;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) o[i] = fmaf(w, (float)v[lane + 32 * i], o[i]);
+  for (int e = 0; e < D / 32; ++e)
+    any = any || ((x.last[e] > pos || x.first[e] <= pos - p.window) && !(x.nan0[e] >= 0 && (seesKey(p, pos, x.nan0[e]) || seesKey(p, pos, x.nan1[e]))));
+  return __any_sync(0xffffffffu, any);
+}
+
+// Sums the rows of `redo` again that may be spoilt, by multiply-adds over the keys that they see: the two warps that share 32 rows call it with their
+// `side` and take every other such row, four rows and four keys at a time, lane l the kEach elements l of a row.  What lane i knows of row i: its place,
+// its query's offset, what its weights are relative to, its factor.  The sums go to `part` of cut keys, else divided and rounded to the tile's
+// outputs in shared memory.
+template <typename T, int D>
+__device__ __noinline__ void mendRows(const ChunkArgs& a, const Plan* plan, int t, int side, int row0, int h, unsigned redo, int pos, long long qOff, float base, float inv,
+                                      uint8_t* tileQ, float* part) {
+  using L = LaneOf<D>;
+  using Pack = typename L::Pack;
+  constexpr int kRows = 4, kBatch = 4, kEach = L::kEach;
+  const PagedArgs& p = a.p;
+  const int lane = threadIdx.x & 31;
+  unsigned mine = 0;
+  {
+    Taint<D> taint;
+    findTaint<T, D>(a, plan, t, h, taint);
+    for (int count = 0; redo; redo &= redo - 1) {
+      const int src = __ffs(redo) - 1;
+      if (spoils<D>(p, taint, __shfl_sync(0xffffffffu, pos, src)) && (count++ & 1) == side) mine |= 1u << src;
+    }
+  }
+  while (mine) {
+    int src[kRows], at[kRows], low = 0x7fffffff, high = -1;
+    float q[kRows][kEach], o[kRows][kEach], minus[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      src[r] = mine ? __ffs(mine) - 1 : src[r > 0 ? r - 1 : 0];   // fewer than four are left: the last one again
+      mine &= mine - 1;
+      at[r] = __shfl_sync(0xffffffffu, pos, src[r]);
+      low = min(low, at[r]);
+      high = max(high, at[r]);
+      minus[r] = -__shfl_sync(0xffffffffu, base, src[r]);
+      unpack<T, D>(reinterpret_cast<const Pack*>(reinterpret_cast<const T*>(p.q) + __shfl_sync(0xffffffffu, qOff, src[r]))[lane], q[r]);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) { q[r][e] *= a.signQ; o[r][e] = 0.f; }
+    }
+    for (int u = plan->begin; u < plan->end; ++u) {
+      const int j0 = keyOf(plan->bl, u, kKeys);
+      const bool whole = j0 + kKeys - 1 <= low && (j0 > high - p.window || j0 + kKeys <= p.sinks);   // every row sees all keys
+      for (int j = j0; j < j0 + kKeys; j += kBatch) {
+        int page[kBatch];
+        Pack k[kBatch], v[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) page[i] = j + i <= high ? (int)pageOf(p, plan->seq, (j + i) >> a.pageShift) : -1;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {              // without branches, so that all are under way: what has no page, from page 0
+          const long long from = page[i] < 0 ? 0 : page[i], slot = (j + i) & ((1 << a.pageShift) - 1);
+          k[i] = reinterpret_cast<const Pack*>(reinterpret_cast<const T*>(p.k) + from * p.kcSp + slot * p.kcSn + h * p.kcSh)[lane];
+          v[i] = reinterpret_cast<const Pack*>(reinterpret_cast<const T*>(p.v) + from * p.vcSp + slot * p.vcSn + h * p.vcSh)[lane];
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          float x[kEach], y[kEach], w[kRows];
+          unpack<T, D>(k[i], x);
+          unpack<T, D>(v[i], y);
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            w[r] = 0.f;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) w[r] = fmaf(x[e], q[r][e], w[r]);
+          }
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) w[r] = exp2Fast(fmaf(warpSum(w[r]), a.scaleAbs, minus[r]));
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            if (page[i] < 0 || !(whole || seesKey(p, at[r], j + i))) continue;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) o[r][e] = fmaf(w[r], y[e], o[r][e]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const float f = __shfl_sync(0xffffffffu, inv, src[r]);
+      const int row = row0 + src[r];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int e = lane * kEach + i;
+        if (part) part[((long long)(e / 4) * kTileRows + row) * 4 + (e & 3)] = o[r][i];
+        else {
+          T* dst = reinterpret_cast<T*>(tileQ + (e >> 6) * Config<D>::kAtom + row * 128 + ((((e >> 3) & 7) ^ (row & 7)) << 4)) + (e & 7);
+          if constexpr (std::is_same<T, __half>::value) *dst = __float2half_rn(o[r][i] * f);
+          else *dst = __float2bfloat16_rn(o[r][i] * f);
+        }
+      }
     }
   }
 }
@@ -628,29 +746,18 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_consta
         }
       }
     }
-    pairBarrier(bar);
     const bool live = liveRow();
     int oHead;
     const int oTok = tokenOf(oHead);
-    unsigned redo = __ballot_sync(0xffffffffu, odd && live && fabsf(l) <= 3.402823466e38f);
-    while (redo) {
-      const int src = __ffs(redo) - 1, rr = q4 * 32 + src;
-      redo &= redo - 1;
-      float o[D / 32];
-      sumRow<T, D>(a, plan->seq, h, __shfl_sync(0xffffffffu, (long long)(plan->qBegin + oTok) * p.qSt + oHead * p.qSh, src), __shfl_sync(0xffffffffu, pos, src), plan->bl, plan->begin, plan->end, __shfl_sync(0xffffffffu, base, src), o);
-      const float f = __shfl_sync(0xffffffffu, inv, src);
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const int e = lane + 32 * i;
-        if (cut) part[((long long)(e / 4) * kTileRows + rr) * 4 + (e & 3)] = o[i];
-        else {
-          T* dst = reinterpret_cast<T*>(tileQ + (e >> 6) * C::kAtom + rr * 128 + ((((e >> 3) & 7) ^ (rr & 7)) << 4)) + (e & 7);
-          if constexpr (std::is_same<T, __half>::value) *dst = __float2half_rn(o[i] * f);
-          else *dst = __float2bfloat16_rn(o[i] * f);
-        }
-      }
+    odd = odd && live && fabsf(l) <= 3.402823466e38f;
+    if (barrierOr(bar, odd)) {
+      // sums that are not finite though their weights are
+      storeShared(mineAt, odd ? 1.f : 0.f);
+      pairBarrier(bar);
+      const unsigned redo = __ballot_sync(0xffffffffu, odd || loadShared(otherAt) != 0.f);
+      mendRows<T, D>(a, plan, t, side, q4 * 32, h, redo, pos, (long long)(plan->qBegin + oTok) * p.qSt + oHead * p.qSh, base, inv, tileQ, cut ? part : nullptr);
+      pairBarrier(bar);
     }
-    pairBarrier(bar);
     if (!cut) {
       const long long oOff = (long long)(plan->qBegin + oTok) * p.oSt + oHead * p.oSh;
 #pragma unroll
