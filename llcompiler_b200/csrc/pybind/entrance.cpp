@@ -276,7 +276,7 @@ Operand output(const char* name, py::object& out, py::handle like, const Operand
 struct Turns { uintptr_t positions = 0, freq = 0; int posType = LLC_INT64, axes = 0; int64_t posStride = 0, pairs = 0; int32_t sections[LLC_ROTARY_MAX_AXES] = {0, 0, 0, 0}; };
 Turns turns(py::handle positions, py::handle freq, py::handle sections, int64_t tokens, int64_t d, int device) {
   Turns t;
-  Operand f("inv_freq", freq, 1, 1, true);
+  Operand f("inv_freq", freq, 1, 1);
   f.on(device);
   f.type(LLC_FLOAT64, "float64");
   f.unit(0, "it");

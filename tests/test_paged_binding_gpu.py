@@ -1,0 +1,44 @@
+"""What the decoder operators' Python calls make of autograd's tensors: nothing that needs a derivative is taken, nothing written unseen."""
+import pytest
+import torch
+
+import paged_reference as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _inputs():
+    k, v, table, q_start, kv_len = (t.to(DEV) for t in R.make_batch([3], [20], 16, 2, 64, torch.bfloat16))
+    bf = dict(device=DEV, dtype=torch.bfloat16)
+    return dict(q=torch.ones(3, 4, 64, **bf), new=torch.ones(3, 2, 64, **bf), k=k, v=v, batch=(table, q_start, kv_len), freq=R.inv_freq(32).to(DEV), pos=torch.arange(3, device=DEV),
+                out=torch.zeros(3, 4, 64, **bf))
+
+
+def _calls():
+    """Every operand of every call that may be of a floating type: name, and the call with that operand changed by `f`."""
+    from llcompiler_b200.executor import kv_append, paged_attention, rotary
+    turn = lambda d: rotary(d["q"], d["pos"], d["freq"], out=d["out"])
+    write = lambda d: kv_append(d["new"], d["new_v"], d["k"], d["v"], *d["batch"], q=d["q"], inv_freq=d["freq"], q_out=d["out"])
+    read = lambda d: paged_attention(d["q"], d["k"], d["v"], *d["batch"], out=d["out"])
+    return [("rotary", turn, ("q", "freq", "out")), ("kv_append", write, ("new", "new_v", "k", "v", "q", "freq", "out")), ("paged_attention", read, ("q", "k", "v", "out"))]
+
+
+CASES = [("rotary", n) for n in ("q", "freq", "out")] + [("kv_append", n) for n in ("new", "new_v", "k", "v", "q", "freq", "out")] + [("paged_attention", n) for n in ("q", "k", "v", "out")]
+
+
+def _call_with(which, name, change):
+    call = {w: c for w, c, _ in _calls()}[which]
+    d = _inputs()
+    d["new_v"] = d["new"].clone()
+    d[name] = change(d[name])
+    return lambda: call(d)
+
+
+@pytest.mark.parametrize("which,name", CASES)
+def test_operands_that_require_a_gradient_are_refused(which, name):
+    call = _call_with(which, name, lambda t: t.clone().requires_grad_())
+    with pytest.raises(ValueError, match="requires a gradient"):
+        call()
+    with torch.no_grad():                                     # nobody asks for it there
+        call()
