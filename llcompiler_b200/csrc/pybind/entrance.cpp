@@ -167,20 +167,25 @@ struct Execution {
 // ---- Operators of the kernel library that a serving loop calls on device tensors directly, without a compiled plan
 // (llcompiler_b200/executor/paged.py).  A decoding step makes a handful of such calls of a few microseconds each, so the checks are
 // made here: what a tensor says of itself is read through the interpreter once, nothing links against the tensor library.
+py::object got(PyObject* o) { if (!o) throw py::error_already_set(); return py::reinterpret_steal<py::object>(o); }
+
 struct Torch {
-  py::object tensor, emptyLike, empty, stream, gradEnabled;
+  py::object tensor, emptyLike, empty, stream, gradEnabled, forwardAd;
   py::object f32, f16, bf16, f64, i32, i64;
-  PyObject* nShape, *nStride, *nDtype, *nPtr, *nDevice, *nGrad, *nDeviceOf, *kwEmpty;
+  PyObject* nShape, *nStride, *nDtype, *nPtr, *nDevice, *nGrad, *nDeviceOf, *nLevel, *kwEmpty;
   Torch() {
     py::module_ t = py::module_::import("torch"), c = py::module_::import("torch._C");
     tensor = t.attr("Tensor"); emptyLike = t.attr("empty_like"); empty = t.attr("empty"); gradEnabled = t.attr("is_grad_enabled");
-    stream = c.attr("_cuda_getCurrentRawStream");
+    stream = c.attr("_cuda_getCurrentRawStream"); forwardAd = py::module_::import("torch.autograd.forward_ad");
     f32 = t.attr("float32"); f16 = t.attr("float16"); bf16 = t.attr("bfloat16"); f64 = t.attr("float64"); i32 = t.attr("int32"); i64 = t.attr("int64");
     nShape = PyUnicode_InternFromString("shape"); nStride = PyUnicode_InternFromString("stride"); nDtype = PyUnicode_InternFromString("dtype");
     nPtr = PyUnicode_InternFromString("data_ptr"); nDevice = PyUnicode_InternFromString("get_device"); nGrad = PyUnicode_InternFromString("requires_grad");
-    nDeviceOf = PyUnicode_InternFromString("device");
+    nDeviceOf = PyUnicode_InternFromString("device"); nLevel = PyUnicode_InternFromString("_current_level");
     kwEmpty = PyTuple_Pack(2, nDtype, nDeviceOf);
   }
+  // Whether a dual level is open (-1: none is): asked once a call, the level is the process's.
+  mutable bool dualLevel = false;
+  void look() const { dualLevel = PyLong_AsLong(got(PyObject_GetAttr(forwardAd.ptr(), nLevel)).ptr()) >= 0; }
   int code(PyObject* d) const {
     if (d == bf16.ptr()) return LLC_BFLOAT16;
     if (d == f16.ptr()) return LLC_FLOAT16;
@@ -192,8 +197,6 @@ struct Torch {
   }
 };
 const Torch& torch() { static Torch* t = new Torch(); return *t; }   // never destroyed: the interpreter may be gone by then
-
-py::object got(PyObject* o) { if (!o) throw py::error_already_set(); return py::reinterpret_steal<py::object>(o); }
 
 int64_t number(const char* name, PyObject* o) {
   const long long x = PyLong_AsLongLong(o);
@@ -228,7 +231,10 @@ struct Operand {
     ptr = (uintptr_t)PyLong_AsUnsignedLongLong(pt.ptr());
     if (PyErr_Occurred()) throw py::error_already_set();
     if (device < 0) bad("expected a CUDA tensor; there is no CPU fallback");
-    if (!index && got(PyObject_GetAttr(o, t.nGrad)).ptr() == Py_True && t.gradEnabled().cast<bool>()) bad("inference only, it requires a gradient");
+    if (index) return;
+    if (got(PyObject_GetAttr(o, t.nGrad)).ptr() == Py_True && t.gradEnabled().cast<bool>()) bad("inference only, it requires a gradient");
+    // a dual tensor does not say so itself
+    if (t.dualLevel && !t.forwardAd.attr("unpack_dual")(h).attr("tangent").is_none()) bad("inference only, it carries a forward-mode tangent");
   }
   // A tensor just made like `l`: only its strides and its address are news.
   Operand(const char* name_, py::handle h, const Operand& l) : name(name_) {
@@ -426,6 +432,7 @@ py::object pagedAttention(py::handle q, py::handle kCache, py::handle vCache, py
 template <Py_ssize_t N, typename F> PyObject* enter(const char* name, Py_ssize_t n, F f) {
   try {
     if (n != N) throw py::type_error(std::string(name) + ": expected " + std::to_string(N) + " arguments, got " + std::to_string(n));
+    torch().look();
     return f().release().ptr();
   } catch (py::error_already_set& e) {
     e.restore();

@@ -42,3 +42,14 @@ def test_operands_that_require_a_gradient_are_refused(which, name):
         call()
     with torch.no_grad():                                     # nobody asks for it there
         call()
+
+
+@pytest.mark.parametrize("which,name", CASES)
+def test_operands_with_a_forward_mode_tangent_are_refused(which, name):
+    """A dual tensor does not require a gradient; its tangent would be lost.  Other tensors are taken inside a dual level."""
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        call = _call_with(which, name, lambda t: fwd.make_dual(t.clone(), torch.ones_like(t)))
+        with pytest.raises(ValueError, match="tangent"):
+            call()
+        _call_with(which, name, lambda t: t)()
