@@ -9,6 +9,7 @@
 
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -170,13 +171,14 @@ struct Execution {
 py::object got(PyObject* o) { if (!o) throw py::error_already_set(); return py::reinterpret_steal<py::object>(o); }
 
 struct Torch {
-  py::object tensor, emptyLike, empty, stream, gradEnabled, forwardAd;
+  py::object tensor, emptyLike, empty, stream, gradEnabled, forwardAd, wrote;
   py::object f32, f16, bf16, f64, i32, i64;
   PyObject* nShape, *nStride, *nDtype, *nPtr, *nDevice, *nGrad, *nDeviceOf, *nLevel, *kwEmpty;
   Torch() {
     py::module_ t = py::module_::import("torch"), c = py::module_::import("torch._C");
     tensor = t.attr("Tensor"); emptyLike = t.attr("empty_like"); empty = t.attr("empty"); gradEnabled = t.attr("is_grad_enabled");
     stream = c.attr("_cuda_getCurrentRawStream"); forwardAd = py::module_::import("torch.autograd.forward_ad");
+    wrote = c.attr("_increment_version");
     f32 = t.attr("float32"); f16 = t.attr("float16"); bf16 = t.attr("bfloat16"); f64 = t.attr("float64"); i32 = t.attr("int32"); i64 = t.attr("int64");
     nShape = PyUnicode_InternFromString("shape"); nStride = PyUnicode_InternFromString("stride"); nDtype = PyUnicode_InternFromString("dtype");
     nPtr = PyUnicode_InternFromString("data_ptr"); nDevice = PyUnicode_InternFromString("get_device"); nGrad = PyUnicode_InternFromString("requires_grad");
@@ -264,8 +266,7 @@ Operand firstRows(const char* name, py::handle h) {
 }
 // The result's tensor: the caller's, or a new one.
 Operand output(const char* name, py::object& out, py::handle like, const Operand& l) {
-  const bool own = out.is_none();
-  if (own) {
+  if (out.is_none()) {
     out = got(PyObject_CallOneArg(torch().emptyLike.ptr(), like.ptr()));
     Operand o(name, out, l);
     if (l.n[2] <= 1 || o.s[2] == 1) return o;
@@ -348,12 +349,20 @@ void* streamOf(int device) {
   py::object d = got(PyLong_FromLong(device)), s = got(PyObject_CallOneArg(torch().stream.ptr(), d.ptr()));
   return PyLong_AsVoidPtr(s.ptr());
 }
+// Tells autograd of the caller's tensors that a call has written: a graph that has saved one of them raises then instead of using new values.
+void wrote(std::initializer_list<PyObject*> tensors) {
+  py::tuple t(tensors.size());
+  Py_ssize_t i = 0;
+  for (PyObject* x : tensors) { Py_INCREF(x); PyTuple_SET_ITEM(t.ptr(), i++, x); }
+  got(PyObject_CallOneArg(torch().wrote.ptr(), t.ptr()));
+}
 template <typename T = void> T* at(uintptr_t p) { return reinterpret_cast<T*>(p); }
 
 py::object rotary(py::handle x, py::handle positions, py::handle freq, py::handle sections, bool interleaved, py::object out) {
   Operand a = firstRows("x", x);
   if (positions.is_none()) throw py::value_error("positions: required");
   const Turns t = turns(positions, freq, sections, a.n[0], a.n[2], a.device);
+  const bool given = !out.is_none();
   const Operand o = output("out", out, x, a);
   LlcRotaryParams p{};
   p.x = at(a.ptr); p.out = at(o.ptr); p.positions = at(t.positions); p.inv_freq = at<const double>(t.freq);
@@ -361,6 +370,7 @@ py::object rotary(py::handle x, py::handle positions, py::handle freq, py::handl
   p.x_st = a.s[0]; p.x_sh = a.s[1]; p.o_st = o.s[0]; p.o_sh = o.s[1]; p.pos_sa = t.posStride; p.axes = t.axes; p.interleaved = interleaved;
   std::memcpy(p.sections, t.sections, sizeof p.sections);
   check(llc_cuda_rotary(&p, streamOf(a.device)));
+  if (given) wrote({out.ptr()});
   return out;
 }
 
@@ -372,12 +382,13 @@ py::object kvAppend(py::handle k, py::handle v, py::handle kCache, py::handle vC
   if (a.n[1] != kc.n[2] || a.n[2] != kc.n[3]) a.bad("expected [tokens, " + std::to_string(kc.n[2]) + ", " + std::to_string(kc.n[3]) + "], got " + a.shape());
   const Batch s = batchOf(table, start, len, bad, a.device);
   LlcKvAppendParams p{};
+  const bool given = !qOut.is_none();
   if (!q.is_none()) {
     Operand x = rowsLike("q", q, a);
     if (x.n[0] != a.n[0] || x.n[2] != a.n[2]) x.bad("expected [" + std::to_string(a.n[0]) + ", heads, " + std::to_string(a.n[2]) + "], got " + x.shape());
     const Operand o = output("q_out", qOut, q, x);
     p.q = at(x.ptr); p.q_out = at(o.ptr); p.heads = x.n[1]; p.q_st = x.s[0]; p.q_sh = x.s[1]; p.qo_st = o.s[0]; p.qo_sh = o.s[1];
-  } else if (!qOut.is_none()) {
+  } else if (given) {
     throw py::value_error("q_out: no queries were given");
   }
   if (!freq.is_none()) {
@@ -392,6 +403,8 @@ py::object kvAppend(py::handle k, py::handle v, py::handle kCache, py::handle vC
   p.table_s0 = s.stride; p.k_st = a.s[0]; p.k_sh = a.s[1]; p.v_st = b.s[0]; p.v_sh = b.s[1];
   p.kc_sp = kc.s[0]; p.kc_sn = kc.s[1]; p.kc_sh = kc.s[2]; p.vc_sp = vc.s[0]; p.vc_sn = vc.s[1]; p.vc_sh = vc.s[2]; p.interleaved = interleaved;
   check(llc_cuda_kv_append(&p, streamOf(a.device)));
+  if (given) wrote({kCache.ptr(), vCache.ptr(), qOut.ptr()});
+  else wrote({kCache.ptr(), vCache.ptr()});
   return qOut;
 }
 
@@ -405,6 +418,7 @@ py::object pagedAttention(py::handle q, py::handle kCache, py::handle vCache, py
   if (window < 0 || sinks < 0) throw py::value_error("window and sinks: must not be negative");
   const int64_t most = maxQ.is_none() ? a.n[0] : number("max_q", maxQ.ptr());
   if (most < 0) throw py::value_error("max_q: must not be negative");
+  const bool given = !out.is_none();
   const Operand o = output("out", out, q, a);
   LlcPagedAttentionParams p{};
   p.q = at(a.ptr); p.k_cache = at(kc.ptr); p.v_cache = at(vc.ptr); p.out = at(o.ptr); p.page_table = s.table; p.q_start = s.start; p.kv_len = s.len; p.bad_pages = s.bad;
@@ -424,6 +438,7 @@ py::object pagedAttention(py::handle q, py::handle kCache, py::handle vCache, py
     p.workspace_bytes = bytes;
   }
   check(llc_cuda_paged_attention(&p, streamOf(a.device)));
+  if (given) wrote({out.ptr()});
   return out;
 }
 

@@ -10,7 +10,8 @@ A cache is a pool of pages, ``k_cache`` and ``v_cache`` of shape ``[num_pages, p
 tensors on the device: ``page_table [batch, width]``, ``q_start [batch + 1]`` (rows of ``q``/``k``/``v`` of each sequence) and
 ``kv_len [batch]`` (tokens in the cache, the new ones included).  The calls read them on the device and enqueue work on
 the current stream of the tensors' device, so a step can be captured into a CUDA graph and replayed with other lengths.
-Rows behind ``q_start[batch]`` are left as they are.  Inference only: a tensor that requires a gradient is refused.
+Rows behind ``q_start[batch]`` are left as they are.  Inference only: a tensor that requires a gradient
+or carries a forward-mode tangent is refused; tensors of the caller's that a call writes count as changed in place.
 
 The reference has no counterpart (its attention is the decomposed chain of llcompiler/compiler/torch_compile_config.py:24
 over dense tensors); the entry points are llc_cuda_rotary, llc_cuda_kv_append and llc_cuda_paged_attention of the C ABI.

@@ -53,3 +53,33 @@ def test_operands_with_a_forward_mode_tangent_are_refused(which, name):
         with pytest.raises(ValueError, match="tangent"):
             call()
         _call_with(which, name, lambda t: t)()
+
+
+@pytest.mark.parametrize("which,name", [("rotary", "out"), ("kv_append", "k"), ("kv_append", "v"), ("kv_append", "out"), ("paged_attention", "out")])
+def test_a_graph_that_saved_what_a_call_writes_raises(which, name):
+    call = {w: c for w, c, _ in _calls()}[which]
+    d = _inputs()
+    d["new_v"] = d["new"].clone()
+    d[name] = d[name].abs() + 1
+    w = torch.ones_like(d[name], requires_grad=True)
+    (w * d[name]).sum().backward()                            # as long as nothing is written
+    graph = (w * d[name]).sum()
+    with torch.no_grad():
+        call(d)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        graph.backward()
+
+
+def test_nothing_else_counts_as_written():
+    d = _inputs()
+    d["new_v"] = d["new"].clone()
+    before = {n: t._version for n, t in d.items() if isinstance(t, torch.Tensor)}
+    from llcompiler_b200.executor import kv_append, paged_attention, rotary
+    made = [rotary(d["q"], d["pos"], d["freq"]), paged_attention(d["q"], d["k"], d["v"], *d["batch"])]
+    assert {n: t._version for n, t in d.items() if isinstance(t, torch.Tensor)} == before
+    made.append(kv_append(d["new"], d["new_v"], d["k"], d["v"], *d["batch"], q=d["q"], inv_freq=d["freq"]))
+    assert all(t._version == 0 for t in made)
+    assert {n for n, t in d.items() if isinstance(t, torch.Tensor) and t._version != before[n]} == {"k", "v"}
+    with torch.inference_mode():                              # tensors without a counter are written all the same
+        x = torch.ones(3, 4, 64, device=DEV, dtype=torch.bfloat16)
+        assert rotary(x, d["pos"], d["freq"], out=x) is x
