@@ -198,7 +198,16 @@ struct Torch {
     return -1;
   }
 };
-const Torch& torch() { static Torch* t = new Torch(); return *t; }   // never destroyed: the interpreter may be gone by then
+// Guarded by the interpreter's lock alone: making one runs Python code, which may hand the lock to another thread, and a thread that waited there for
+// a C++ guard would keep it.  Two first calls at once make two, of which one is kept.  Never destroyed: the interpreter may be gone by then.
+const Torch& torch() {
+  static Torch* t = nullptr;
+  if (!t) {
+    Torch* made = new Torch();
+    if (!t) t = made;
+  }
+  return *t;
+}
 
 int64_t number(const char* name, PyObject* o) {
   const long long x = PyLong_AsLongLong(o);
