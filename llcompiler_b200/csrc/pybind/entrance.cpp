@@ -258,6 +258,7 @@ struct Operand {
   }
   void on(int dev) const { if (device != dev) bad("on cuda:" + std::to_string(device) + ", expected cuda:" + std::to_string(dev)); }
   void type(int want, const char* said) const { if (dtype != want) bad(std::string("expected ") + said); }
+  void written() const { for (int i = 0; i < rank; ++i) if (n[i] > 1 && s[i] == 0) bad("an output may not repeat its elements (stride 0)"); }
   void unit(int dim, const char* what) const { if (n[dim] > 1 && s[dim] != 1) bad(std::string(what) + " must have unit stride"); }
 };
 // [tokens, heads, head_dim]
@@ -282,10 +283,8 @@ Operand output(const char* name, py::object& out, py::handle like, const Operand
     out = torch().empty(like.attr("shape"), py::arg("dtype") = like.attr("dtype"), py::arg("device") = like.attr("device"));
   }
   Operand o = rowsLike(name, out, l);
-  for (int i = 0; i < 3; ++i) {
-    if (o.n[i] != l.n[i]) o.bad("expected shape " + l.shape() + ", got " + o.shape());
-    if (o.n[i] > 1 && o.s[i] == 0) o.bad("an output may not repeat its elements (stride 0)");
-  }
+  for (int i = 0; i < 3; ++i) if (o.n[i] != l.n[i]) o.bad("expected shape " + l.shape() + ", got " + o.shape());
+  o.written();
   return o;
 }
 
@@ -388,6 +387,8 @@ py::object kvAppend(py::handle k, py::handle v, py::handle kCache, py::handle vC
   Operand a = firstRows("k", k), b = rowsLike("v", v, a), kc = cacheOf("k_cache", kCache, a), vc = cacheOf("v_cache", vCache, a);
   sameShape(a, b);
   sameShape(kc, vc);
+  kc.written();
+  vc.written();
   if (a.n[1] != kc.n[2] || a.n[2] != kc.n[3]) a.bad("expected [tokens, " + std::to_string(kc.n[2]) + ", " + std::to_string(kc.n[3]) + "], got " + a.shape());
   const Batch s = batchOf(table, start, len, bad, a.device);
   LlcKvAppendParams p{};

@@ -46,7 +46,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sec
     ``positions`` is ``[tokens]`` or ``[axes, tokens]`` (int32 or int64); ``inv_freq`` holds one float64 frequency per pair, and
     ``sections`` says how many pairs belong to each axis, in order (time, height, width of a video, say; default: one axis).
     Pair i is elements ``(i, i + pairs)``, or ``(2i, 2i + 1)`` when ``interleaved``; elements past the pairs are copied.
-    ``out`` may be ``x`` itself."""
+    ``out`` may be ``x`` itself, and shares no memory with it otherwise."""
     if isinstance(x, torch.Tensor) and x.is_cuda and x.get_device() == _current():
         return _ops.rotary(x, positions, inv_freq, sections, interleaved, out)
     return _elsewhere(_ops.rotary, x, positions, inv_freq, sections, interleaved, out)
@@ -61,7 +61,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     With ``inv_freq`` the keys are turned on the way (see ``rotary``; ``positions`` default to the tokens' places in their
     sequences), and so are the queries ``q [tokens, heads, head_dim]``, which are returned (``q_out``, or a new tensor; rows
     of no sequence are not written).  A token whose page number is no page of the pool, or whose place lies outside the
-    table, is not stored and is counted in ``bad_pages`` (one int32) if that is given.  Two tokens must not share a slot."""
+    table, is not stored and is counted in ``bad_pages`` (one int32) if that is given.  Two tokens must not share a slot.
+    ``q_out`` may be ``q`` itself; nothing else that the call writes may lie in memory that it reads or writes otherwise."""
     if isinstance(k, torch.Tensor) and k.is_cuda and k.get_device() == _current():
         return _ops.kv_append(k, v, k_cache, v_cache, page_table, q_start, kv_len, q, positions, inv_freq, sections, interleaved, q_out, bad_pages)
     return _elsewhere(_ops.kv_append, k, v, k_cache, v_cache, page_table, q_start, kv_len, q, positions, inv_freq, sections, interleaved, q_out, bad_pages)
@@ -77,7 +78,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``1 / sqrt(head_dim)``.  ``max_q`` bounds the new tokens of one sequence (default: all of them); a decoding step says 1,
     which lets the call choose the kernel for few rows; a sequence that has more is left out.  A token that sees nothing gets
     zeros, one whose visible scores are all -inf NaN (0 / 0); rows of no sequence are not written.  Pages that are none of the pool's
-    read as zeros and are counted in ``bad_pages`` (one int32) if that is given."""
+    read as zeros and are counted in ``bad_pages`` (one int32) if that is given.  ``out`` may be ``q`` itself, and shares no memory with
+    the operands otherwise."""
     if isinstance(q, torch.Tensor) and q.is_cuda and q.get_device() == _current():
         return _ops.paged_attention(q, k_cache, v_cache, page_table, q_start, kv_len, scale, window, sinks, max_q, out, bad_pages)
     return _elsewhere(_ops.paged_attention, q, k_cache, v_cache, page_table, q_start, kv_len, scale, window, sinks, max_q, out, bad_pages)

@@ -83,3 +83,15 @@ def test_nothing_else_counts_as_written():
     with torch.inference_mode():                              # tensors without a counter are written all the same
         x = torch.ones(3, 4, 64, device=DEV, dtype=torch.bfloat16)
         assert rotary(x, d["pos"], d["freq"], out=x) is x
+
+
+def test_caches_that_repeat_their_elements_are_read_but_not_written():
+    from llcompiler_b200.executor import kv_append, paged_attention
+    d = _inputs()
+    for k, v in ((d["k"][:, :, :1].expand(-1, -1, 2, -1), d["v"]), (d["k"], d["v"][:1].expand(d["v"].shape))):
+        with pytest.raises(ValueError):
+            kv_append(d["new"], d["new"], k, v, *d["batch"])
+        host = [t.cpu() for t in (d["q"], k, v, *d["batch"])]
+        want, size, largest = R.attention(*host, R.scale_of(64), 0, 0)
+        off = (paged_attention(d["q"], k, v, *d["batch"]).double().cpu() - want).abs()
+        assert (off <= R.attention_tolerance(want, size, largest, torch.bfloat16)).all()
