@@ -542,5 +542,6 @@ PYBIND11_MODULE(llcompiler_, m) {
       .def("last_launch_count", &Execution::last_launch_count).def("arena_bytes", &Execution::arena_bytes);
   auto ops = m.def_submodule("ops");
   for (PyMethodDef& f : kOps) ops.attr(f.ml_name) = got(PyCFunction_NewEx(&f, nullptr, nullptr));
+  ops.def("status", []() { return llc_cuda_status(); }, py::call_guard<py::gil_scoped_release>());
   m.def("version", []() { return std::string(llc_version()); });
 }

@@ -83,3 +83,21 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if isinstance(q, torch.Tensor) and q.is_cuda and q.get_device() == _current():
         return _ops.paged_attention(q, k_cache, v_cache, page_table, q_start, kv_len, scale, window, sinks, max_q, out, bad_pages)
     return _elsewhere(_ops.paged_attention, q, k_cache, v_cache, page_table, q_start, kv_len, scale, window, sinks, max_q, out, bad_pages)
+
+
+def device_status(device: Optional[int] = None) -> int:
+    """Waits for the device (default: the current one) and raises if a kernel of an earlier call recorded a failure, which it cannot
+    raise itself: a wait of a tensor-core kernel that gave up, so that its output is wrong.  Returns 0 otherwise.  Reading clears
+    what was recorded.  The calls above return before their kernels have run; a caller asks here after its own synchronisation, as
+    ``Torch_ExecutionEngine.status`` does for compiled plans.  Not to be called while a stream is being captured."""
+    if device is None:
+        code = _ops.status()
+    else:
+        with torch.cuda.device(device):
+            code = _ops.status()
+    if code < 0:
+        raise RuntimeError("device_status: the device cannot be read")
+    if code:
+        who = "attention over the paged cache" if code >= 8 else "attention" if code >= 6 else "a matrix product or convolution"
+        raise RuntimeError(f"device_status: a kernel of {who} gave up (code {code}); its output is wrong")
+    return code

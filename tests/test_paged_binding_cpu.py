@@ -2,6 +2,9 @@
 import os
 import subprocess
 import sys
+import types
+
+import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -26,3 +29,13 @@ for t in threads: t.join()
 def test_first_calls_of_several_threads_at_once():
     r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and r.stdout.split() == ["refused"] * 3, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("code,said", [(-1, "cannot be read"), (2, "matrix product"), (7, "of attention"), (9, "paged cache"), (12, "paged cache .* 12")])
+def test_a_failure_that_a_kernel_recorded_is_raised(monkeypatch, code, said):
+    from llcompiler_b200.executor import device_status, paged
+    monkeypatch.setattr(paged, "_ops", types.SimpleNamespace(status=lambda: code))
+    with pytest.raises(RuntimeError, match=said):
+        device_status()
+    monkeypatch.setattr(paged, "_ops", types.SimpleNamespace(status=lambda: 0))
+    assert device_status() == 0

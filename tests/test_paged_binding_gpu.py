@@ -95,3 +95,12 @@ def test_caches_that_repeat_their_elements_are_read_but_not_written():
         want, size, largest = R.attention(*host, R.scale_of(64), 0, 0)
         off = (paged_attention(d["q"], k, v, *d["batch"]).double().cpu() - want).abs()
         assert (off <= R.attention_tolerance(want, size, largest, torch.bfloat16)).all()
+
+
+def test_the_device_status_is_healthy_after_the_calls():
+    from llcompiler_b200.executor import device_status
+    for _, call, _ in _calls():
+        d = _inputs()
+        d["new_v"] = d["new"].clone()
+        call(d)
+        assert device_status() == 0 and device_status(torch.cuda.current_device()) == 0
