@@ -28,7 +28,7 @@ for t in threads: t.join()
 
 def test_first_calls_of_several_threads_at_once():
     r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=100)
-    assert r.returncode == 0 and r.stdout.split() == ["refused"] * 3, r.stderr[-2000:]
+    assert r.returncode == 0 and r.stdout.count("refused") == 3, r.stderr[-2000:]
 
 
 @pytest.mark.parametrize("code,said", [(-1, "cannot be read"), (2, "matrix product"), (7, "of attention"), (9, "paged cache"), (12, "paged cache .* 12")])
