@@ -49,8 +49,12 @@ struct DecodeArgs {
   int slotRows;                // rows of a slot: the most that a sequence of this call has
   int joinRows;                // rows of a block of the joining kernel
   int2* records;               // [pairs]: first warp of the pair, number of warps that have a part of it
-  float* slots;                // [pairs + warps][slotRows][D + kTail]: a part's sums; slot = pair + warp
+  float* slots;                // [2 x warps][slotRows][D + kTail]: a part's sums, see slotOf
+  int warps;                   // of the grid
 };
+// A share's ends cut two pairs at most: the one that a warp before it has begun, and the last one that it begins itself.
+constexpr int kCutsOfAShare = 2;
+__device__ __forceinline__ long long slotOf(const DecodeArgs& a, int warp, bool begun) { return begun ? warp : (long long)a.warps + warp; }
 
 // The blocks of keys of one key head of a sequence; one empty block where nothing is visible, which writes the zeros; none where the
 // sequence has no rows, or more than this kernel takes.
@@ -386,7 +390,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
       const bool whole = begin == 0 && use.end == use.bl.count;
       const long long pair = (long long)use.b * p.kvHeads + use.h;
       if (begin == 0 && lane == 0) a.records[pair] = make_int2((int)me, 1 + (int)((use.bl.count - use.end + share - 1) / share));
-      float* slot = a.slots + (pair + me) * a.slotRows * (D + kTail);
+      float* slot = a.slots + slotOf(a, (int)me, begin != 0) * a.slotRows * (D + kTail);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -484,15 +488,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
   if (s.n == 0 || (long long)s.n * p.group > C::kRows || row0 >= rows || rec.y < 2) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = rec.y;
   const long long stride = (long long)a.slotRows * (D + kTail);
+  // A row's sums in part n: the first warp has begun the pair, the ones behind it go on with it.
+  auto partAt = [&](int row, int n) { return a.slots + slotOf(a, rec.x + n, n > 0) * stride + row * (D + kTail); };
   // Sums the parts first, first + step, ... of a row with factors that `factor` knows.
-  auto add = [&](const float* part, int first, int step, float* x, auto factor) {
+  auto add = [&](int row, int first, int step, float* x, auto factor) {
 #pragma unroll 1
     for (int i = first; i < parts; i += 8 * step) {
       V v[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int n = i + u * step;
-        if (n < parts) v[u] = reinterpret_cast<const V*>(part + n * stride)[lane];
+        if (n < parts) v[u] = reinterpret_cast<const V*>(partAt(row, n))[lane];
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
@@ -512,30 +518,28 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
   if (a.joinRows > 1 && parts <= 32) {
     const int row = row0 + warp;
     if (row >= rows) return;
-    const float* part = a.slots + ((long long)pair + rec.x) * stride + row * (D + kTail);
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (lane < parts) ml = *reinterpret_cast<const float2*>(part + lane * stride + D);
+    if (lane < parts) ml = *reinterpret_cast<const float2*>(partAt(row, lane) + D);
     const float top = warpMax(ml.x), f = ml.x == -INFINITY ? 0.f : exp2Fast(ml.x - top), total = warpSum(ml.y * f), inv = 1.f / divisorOf(total, top, sees(row));
     float x[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) x[e] = 0.f;
-    add(part, 0, 1, x, [&](int n) { return __shfl_sync(0xffffffffu, f, n); });
+    add(row, 0, 1, x, [&](int n) { return __shfl_sync(0xffffffffu, f, n); });
     T* dst = place(row) + lane * kEach;
     if constexpr (kEach == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv));
     else *reinterpret_cast<uint32_t*>(dst) = pack2<T>(x[0] * inv, x[1] * inv);
     return;
   }
   for (int row = row0; row < row0 + a.joinRows && row < rows; ++row) {
-    const float* part = a.slots + ((long long)pair + rec.x) * stride + row * (D + kTail);
     float top = -INFINITY, sum = 0.f;
-    for (int i = threadIdx.x; i < parts; i += kJoinWarps * 32) top = fmaxf(top, part[i * stride + D]);
+    for (int i = threadIdx.x; i < parts; i += kJoinWarps * 32) top = fmaxf(top, partAt(row, i)[D]);
     top = warpMax(top);
     if (lane == 0) sTop[warp] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, sTop[w]);
     for (int i = threadIdx.x; i < parts; i += kJoinWarps * 32) {
-      const float2 ml = *reinterpret_cast<const float2*>(part + i * stride + D);
+      const float2 ml = *reinterpret_cast<const float2*>(partAt(row, i) + D);
       const float f = ml.x == -INFINITY ? 0.f : exp2Fast(ml.x - top);
       sF[i] = f;
       sum += ml.y * f;
@@ -546,7 +550,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
     float x[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) x[e] = 0.f;
-    add(part, warp, kJoinWarps, x, [&](int n) { return sF[n]; });
+    add(row, warp, kJoinWarps, x, [&](int n) { return sF[n]; });
 #pragma unroll
     for (int e = 0; e < kEach; ++e) sO[warp][lane * kEach + e] = x[e];
     __syncthreads();
@@ -573,7 +577,7 @@ template <int D, int MT> Launch launchOf(const PagedArgs& p) {
   const bool whole = longest <= 512 && pairs <= 2 * slots && pairs * longest <= 512 * slots;
   Launch l{!whole, 0, (int)(rows < MT * 16 ? rows : MT * 16), 0};
   l.ctas = (unsigned)(l.split ? slots : pairs);
-  if (l.split) l.bytes = ((pairs * 8 + 15) & ~15LL) + (pairs + slots * kWarps) * l.rows * (D + kTail) * 4;
+  if (l.split) l.bytes = ((pairs * 8 + 15) & ~15LL) + kCutsOfAShare * slots * kWarps * l.rows * (D + kTail) * 4;
   return l;
 }
 
@@ -604,6 +608,7 @@ int launch(const PagedArgs& p, void* workspace, long long bytes, cudaStream_t st
   if (!l.split || !workspace || bytes < l.bytes) return launchMain<T, D, MT, false>(mk, mv, a, (unsigned)pairs, st);
   a.minBlocks = 4;
   a.slotRows = l.rows;
+  a.warps = (int)l.ctas * kWarps;
   a.records = static_cast<int2*>(workspace);
   a.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((pairs * 8 + 15) & ~15LL));
   if (int rc = launchMain<T, D, MT, true>(mk, mv, a, l.ctas, st)) return rc;
