@@ -168,3 +168,96 @@ def test_values_that_are_not_finite_do_not_stop_a_chunk(where):
     assert out.isnan().all() if where == "every" else out[..., 7].isinf().all() if where == "early" else out[40:, :, 7].isinf().all() and torch.isfinite(out[:40].float()).all()
     slow = _ms(lambda: paged_attention(q, k, v, table, q_start, kv_len), 3)
     assert slow < 4 * clean + (0.05 if where != "chunk" else 10.0), (clean, slow)
+
+
+def _tight_tolerance(want, size, largest, dtype):
+    """R.attention_tolerance without the polynomial exponentials, which only the chunk kernel has: one rounding of the result and one of each
+    weight (16-bit types), scores off by at most d 2^-23 of the largest sum |q k|, twice, and 2^-18 for the hardware's exponential
+    and the sums of weights."""
+    u, d = torch.finfo(dtype).eps / 2, want.shape[-1]
+    return want.abs() * u * (1 + 2.0 ** -7) + size * (u + 2 * largest * d * 2.0 ** -23 + 2.0 ** -18) + 1e-30 + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+
+
+@pytest.mark.parametrize("new,lens,heads,kv_heads,d,page,dtype", [
+    ([1, 1, 1], [1, 64, 300], 8, 2, 128, 16, torch.float16), ([1, 1], [5000, 700], 4, 1, 64, 64, torch.float16), ([2, 3], [517, 90], 10, 2, 128, 32, torch.float16),
+    ([1, 4], [1300, 64], 8, 1, 64, 16, torch.bfloat16), ([3, 1], [50, 400], 4, 2, 64, 16, torch.float32), ([2], [900], 4, 2, 128, 16, torch.float32),
+    ([3, 1], [50, 400], 4, 2, 80, 16, torch.float16), ([2], [200], 2, 1, 256, 16, torch.float32)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 5)])
+def test_decoding_and_plain_kernels_keep_the_bound_without_polynomials(new, lens, heads, kv_heads, d, page, dtype, window, sinks):
+    k, v, table, q_start, kv_len = R.make_batch(new, lens, page, kv_heads, d, dtype, fill=float("nan"))
+    q = _q(sum(new), heads, d, dtype)
+    got = _run(q, k, v, table, q_start, kv_len, window, sinks, max_q=max(new))
+    want, size, largest = R.attention(q, k, v, table, q_start, kv_len, R.scale_of(d), window, sinks)
+    off, tol = (got.double().cpu() - want).abs(), _tight_tolerance(want, size, largest, dtype)
+    assert (off <= tol).all(), float((off / tol).max())
+
+
+@pytest.mark.parametrize("new,lens,heads,kv_heads,width", [
+    ([1, 40, 1], [300, 200, 77], 20, 1, 300), ([1, 3, 1, 0], [4700, 60, 5, 9], 32, 1, 300), ([1, 50, 2], [90, 60, 40], 34, 2, 260),      # 17 to 32 heads, beside chunks
+    ([1], [77], 40, 1, 5), ([1, 1, 50], [300, 5, 60], 40, 1, 300), ([2, 1], [300, 200], 66, 2, 300), ([1, 2], [2000, 31], 128, 1, 130)])  # more than 32
+@pytest.mark.parametrize("d", [64, 128])
+def test_wide_groups(new, lens, heads, kv_heads, width, d):
+    k, v, table, q_start, kv_len = R.make_batch(new, lens, 16, kv_heads, d, torch.bfloat16, width=width, fill=float("nan"))
+    q = _q(sum(new) + 2, heads, d, torch.bfloat16)
+    for window, sinks in ((0, 0), (30, 4)):
+        out = torch.full(q.shape, 5.0, device=DEV, dtype=torch.bfloat16)
+        _run(q, k, v, table, q_start, kv_len, window, sinks, max_q=max(new), out=out)
+        assert (out[sum(new) :] == 5).all()
+        _against_definition(out, q, k, v, table, q_start, kv_len, window, sinks)
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_captured_chunks_replay_with_other_lengths(dtype, d):
+    """A step of chunks captured once: replayed with longer and shorter caches (cut and not), other shares of the rows, and rows of nobody."""
+    from llcompiler_b200.executor import paged_attention
+    rows, heads, kv_heads, page, max_q = 96, 4, 2, 16, 70
+    k, v, table, _, _ = R.make_batch([1, 1, 1], [5000, 5000, 400], page, kv_heads, d, dtype)
+    dev = [t.to(DEV) for t in (k, v, table)]
+    q = _q(rows, heads, d, dtype).to(DEV)
+    q_start, kv_len = torch.tensor([0, 40, 70, 96], dtype=torch.int32, device=DEV), torch.tensor([60, 300, 26], dtype=torch.int32, device=DEV)
+    out = torch.empty_like(q)
+    step = lambda: paged_attention(q, *dev, q_start, kv_len, max_q=max_q, out=out)
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for ends, lens in (([0, 40, 70, 96], [60, 300, 26]), ([0, 70, 70, 70], [5000, 9, 400]), ([0, 33, 66, 90], [4990, 4991, 33]), ([3, 4, 5, 40], [900, 5000, 300]), ([0, 0, 0, 0], [0, 5, 9])):
+        q_start.copy_(torch.tensor(ends, dtype=torch.int32))
+        kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+        q.copy_(_q(rows, heads, d, dtype, seed=sum(lens)))
+        out.fill_(5.0)
+        g.replay()
+        torch.cuda.synchronize()
+        owned = _owned(q_start.cpu(), rows)
+        assert (out.cpu()[~owned] == 5).all()
+        _against_definition(out, q.cpu(), k, v, table, q_start.cpu(), kv_len.cpu())
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_two_runs_give_the_same_bits(form):
+    new, lens, heads, kv_heads, d, page, dtype = FORMS[form]
+    k, v, table, q_start, kv_len = R.make_batch(new, lens, page, kv_heads, d, dtype)
+    q = _q(sum(new), heads, d, dtype)
+    first = _run(q, k, v, table, q_start, kv_len, max_q=max(new))
+    for _ in range(5):
+        assert torch.equal(_run(q, k, v, table, q_start, kv_len, max_q=max(new)), first)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_tensors_of_another_device_than_the_current_one():
+    from llcompiler_b200.executor import device_status, kv_append, paged_attention, rotary
+    other = torch.device("cuda", 1)
+    for new, lens in (([1, 1], [300, 77]), ([40], [300])):
+        k, v, table, q_start, kv_len = R.make_batch(new, lens, 16, 2, 64, torch.bfloat16)
+        q = _q(sum(new), 4, 64, torch.bfloat16)
+        kc, vc = k.to(other), v.to(other)
+        args = [t.to(other) for t in (table, q_start, kv_len)]
+        fresh = _q(sum(new), 2, 64, torch.bfloat16, seed=2)
+        kv_append(fresh.to(other), fresh.to(other), kc, vc, *args)
+        got = paged_attention(q.to(other), kc, vc, *args, max_q=max(new))
+        assert got.device == other and torch.cuda.current_device() == 0
+        _against_definition(got, q, kc.cpu(), vc.cpu(), table, q_start, kv_len)
+        pos, freq = torch.arange(sum(new)), R.inv_freq(32)
+        assert torch.equal(rotary(q.to(other), pos.to(other), freq.to(other)).cpu(), rotary(q.to(DEV), pos.to(DEV), freq.to(DEV)).cpu())
+        assert device_status(other) == 0
