@@ -1,6 +1,7 @@
 // Host side of the tensor-core GEMM and convolution: tensor maps, the choice of tile, the calls that go there.
 // The kernel is in gemm_tc_kernel.cuh, its instantiations in gemm_tc_{dense,im2col}_*.cu and gemm_tc_gather.cu.
 #include "gemm_tc_kernel.cuh"
+#include "tensor_map.h"
 
 namespace llc {
 
@@ -22,19 +23,6 @@ namespace {
 using namespace tcgemm;
 
 // ---- host side ------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encodeTiled() {
-  static EncodeTiledFn fn = []() -> EncodeTiledFn {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
-    return reinterpret_cast<EncodeTiledFn>(p);
-  }();
-  return fn;
-}
-
 // K-major operand [b0, b1, rows, K] with unit stride along K -> 4-D tensor map, box = 128 bytes of K x boxRows rows.
 bool makeMap(CUtensorMap* map, const void* base, bool f32, long long K, long long rows, long long b1, long long b0, long long sRow, long long s1,
              long long s0, int boxRows) {

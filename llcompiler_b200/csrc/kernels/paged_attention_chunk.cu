@@ -15,9 +15,9 @@
 // Bound: at d = 128 a block of two tiles costs 2048 cycles of products and as many of exponentials (16 a cycle and SM); it takes 3460, a
 // tile's chain score -> weight -> sum -> next score, of which the other tile's fills a part.  Measured: 1.8 - 2.0 us a block (1250 to 1390
 // TFLOP/s in the steady state), 4096 tokens over 16384 keys of 32 heads of 128 0.87 ms (1110 TFLOP/s), d = 64 1.5 - 1.6 us a block.
+#include "page_map.h"
 #include "paged_attention.cuh"
 #include "tc_common.cuh"
-#include "tensor_map.h"
 
 namespace llc {
 __device__ int g_pagedChunkStatus = 0;    // non-zero after a bounded wait gave up: 10 loader, 11 issuer, 12 softmax

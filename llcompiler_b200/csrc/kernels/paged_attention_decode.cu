@@ -12,9 +12,9 @@
 // (launched early, it waits for this one on the device).  Few and short pairs (SPLIT false) take a CTA each instead, whose warps
 // take the blocks in turn and meet in shared memory: the second launch costs more than it saves there.
 // Before this, four warps shared blocks of 64 keys and met at the end of every pair: 10000 cycles from one pair to the next.
+#include "page_map.h"
 #include "paged_attention.cuh"
 #include "tc_common.cuh"
-#include "tensor_map.h"
 
 namespace llc {
 __device__ int g_pagedDecodeStatus = 0;   // non-zero after a bounded wait gave up: 8; 9: misplaced shared memory
