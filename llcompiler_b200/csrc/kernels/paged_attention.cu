@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedArgs
   const int b = sSeq;
   if (b >= p.batch || t < p.qStart[b]) return;         // a row of nobody
   const Sequence s = sequenceOf(p, b);
-  if (s.n == 0) return;
+  if (t - s.begin >= s.n) return;                      // none of its rows: starts that do not grow would name places past the table
   const long long pos = s.len - s.n + (t - s.begin);
   const long long lo = pos + 1 - p.window > 0 ? pos + 1 - p.window : 0, first = p.sinks < lo ? p.sinks : lo;
   const long long keys = pos < 0 ? 0 : first + (pos + 1 - lo);

@@ -261,3 +261,36 @@ def test_tensors_of_another_device_than_the_current_one():
         pos, freq = torch.arange(sum(new)), R.inv_freq(32)
         assert torch.equal(rotary(q.to(other), pos.to(other), freq.to(other)).cpu(), rotary(q.to(DEV), pos.to(DEV), freq.to(DEV)).cpu())
         assert device_status(other) == 0
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_row_starts_that_do_not_grow_stay_inside(form):
+    """Starts in any order name no rows, the wrong ones or the same ones twice; places stay inside the table and rows inside the tensors."""
+    from llcompiler_b200.executor import kv_append
+    _, _, heads, kv_heads, d, page, dtype = FORMS[form]
+    reach = 4 * page                                          # every sequence fills its row of the table, the last one at the table's end
+    k, v, table, _, kv_len = R.make_batch([1, 1, 1], [reach] * 3, page, kv_heads, d, dtype, spare=0)
+    q = _q(8, heads, d, dtype)
+    fresh = _q(8, kv_heads, d, dtype, seed=3).to(DEV)
+    for starts in ([0, 9, 1, 2], [0, 8, 1, 2], [5, 2, 7, 1], [0, 1, 0, 8], [-4, 3, -9, 100], [8, 8, 0, 0], [7, -1, 6, 2]):
+        for max_q in (1, 3, 8):
+            out = torch.full(q.shape, 5.0, device=DEV, dtype=dtype)
+            _run(q, k, v, table, torch.tensor(starts, dtype=torch.int32), kv_len, max_q=max_q, out=out)
+            assert torch.isfinite(out.float()).all()
+        dev = [R.to_device(t, DEV) for t in (k, v, table, torch.tensor(starts, dtype=torch.int32), kv_len)]
+        kv_append(fresh, fresh, *dev, bad_pages=torch.zeros(1, device=DEV, dtype=torch.int32))
+        assert torch.isfinite(dev[0].float()).all()
+
+
+@pytest.mark.parametrize("form", [f for f in FORMS if f != "decode_cut_long"])
+def test_rows_that_see_plus_infinity_are_nan(form):
+    """inf - inf, as softmax has it: whichever block or part the score is in, beside finite ones and beside -inf."""
+    new, lens, heads, kv_heads, d, page, dtype = FORMS[form]
+    for at in (0, lens[0] // 2, lens[0] - 1):
+        k, v, table, q_start, kv_len = R.make_batch(new, lens, page, kv_heads, d, dtype)
+        q = _q(sum(new), heads, d, dtype).abs()
+        k[int(table[0, at // page]), at % page] = float("inf")
+        if at:
+            k[int(table[0, 0]), 0] = float("-inf")
+        got = _run(q, k, v, table, q_start, kv_len, max_q=max(new))
+        _against_definition(got, q, k, v, table, q_start, kv_len)
