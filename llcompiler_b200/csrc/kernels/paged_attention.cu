@@ -148,8 +148,11 @@ bool tensorTypes(const PagedArgs& a) {
 int decodeRows(const PagedArgs& a) {
   const long long rows = a.maxQ * a.group;
   if (rows <= 32) return rows <= 16 ? 16 : 32;
-  // few sequences of few keys fit beside the chunks' tiles, and a launch less is worth more (nine sequences of up to 2048 keys, one of them
-  // a single token: 35 us with one kernel, 47 with both)
+  // few sequences of few keys fit beside the chunks' tiles, and launches less are worth more.  One kernel against both, us: nine sequences of up to
+  // 2048 keys, one of them a single token 32 / 43; 16 single tokens and two chunks of 40 over 1000 keys 24 / 41; 60 single tokens and four chunks of
+  // 100 over 1000 keys (2 key heads) 21 / 35; eight single tokens over 3500 keys and eight chunks of 64 over 1500 55 / 70.  At the border the
+  // other way round: 12 single tokens and four chunks of 200 over 4000 keys 124 / 115; past it 24 single tokens and eight chunks of 128 over 2000
+  // keys (256 pairs) 103 / 88, three single tokens and a chunk of 256 over 16000 keys 184 / 181.
   const long long seen = (long long)a.window + a.sinks < a.reach ? (long long)a.window + a.sinks : a.reach;   // keys that a token can see
   if (a.batch == 1 || (seen <= 4096 && a.batch * a.kvHeads <= deviceSMs())) return 0;
   return a.group <= 16 ? 16 : a.group <= 32 ? 32 : 0;

@@ -14,7 +14,8 @@
 // S_A may overwrite P_A as soon as O_A += P_A V has been issued.
 // Bound: at d = 128 a block of two tiles costs 2048 cycles of products and as many of exponentials (16 a cycle and SM); it takes 3460, a
 // tile's chain score -> weight -> sum -> next score, of which the other tile's fills a part.  Measured: 1.8 - 2.0 us a block (1250 to 1390
-// TFLOP/s in the steady state), 4096 tokens over 16384 keys of 32 heads of 128 0.87 ms (1110 TFLOP/s), d = 64 1.5 - 1.6 us a block.
+// TFLOP/s in the steady state), 4096 tokens over 16384 keys of 32 heads of 128 0.86 ms (1120 TFLOP/s) after a pause and 0.94 - 0.97 ms (1000 TFLOP/s) call
+// after call, under the power cap; d = 64 1.5 - 1.6 us a block.
 #include "page_map.h"
 #include "paged_attention.cuh"
 #include "tc_common.cuh"

@@ -11,6 +11,8 @@
 // eight warps an SM).  A pair that a share's end cuts leaves its parts' sums in the workspace, which a second kernel joins
 // (launched early, it waits for this one on the device).  Few and short pairs (SPLIT false) take a CTA each instead, whose warps
 // take the blocks in turn and meet in shared memory: the second launch costs more than it saves there.
+// 17 to 32 rows at d = 128: two tiles of queries, scores and sums in a warp are more than 255 registers (176 bytes of a thread in memory in bf16 and f16,
+// 32 at d = 64), 32 x 8192 keys for 4 tokens of 8 heads a key head 259 us with L2 flushed, floor 164.
 // Before this, four warps shared blocks of 64 keys and met at the end of every pair: 10000 cycles from one pair to the next.
 #include "page_map.h"
 #include "paged_attention.cuh"
@@ -573,7 +575,10 @@ template <int D, int MT> Launch launchOf(const PagedArgs& p) {
   long long longest = p.reach;                     // keys that a sequence can see
   if ((long long)p.window + p.sinks + MT * 16 < longest) longest = (long long)p.window + p.sinks + MT * 16;
   const long long rows = p.maxQ * p.group;
-  // a CTA a pair: up to 512 keys each, and no more work than one such pair a CTA, in at most two rounds of CTAs
+  // a CTA a pair: up to 512 keys each, and no more work than one such pair a CTA, in at most two rounds of CTAs.  Against shares and a second
+  // launch, us, 8 key heads of 128: one sequence of 256 / 512 / 1024 keys 7.5 / 12.1 / 21.4 and 11.3 / 11.6 / 11.9; 16 sequences 8 / 12.7 / 22 and
+  // 14.6 / 15.3 / 20; 64 sequences of 256 keys 16.1 and 18.8, of 512 29.7 and 32.6 (which the third condition leaves to the shares: a ragged
+  // batch would load its CTAs unevenly)
   const bool whole = longest <= 512 && pairs <= 2 * slots && pairs * longest <= 512 * slots;
   Launch l{!whole, 0, (int)(rows < MT * 16 ? rows : MT * 16), 0};
   l.ctas = (unsigned)(l.split ? slots : pairs);

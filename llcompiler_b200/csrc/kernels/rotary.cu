@@ -6,7 +6,8 @@
 // 64-bit product, its whole part is dropped there, and only the fraction (at most half a turn) becomes a float.
 // Bound: memory; every element is read once and written once.  The sine and cosine of a (token, pair) are computed once per
 // block into shared memory and used by all heads of the token; the block's loads of x are under way meanwhile.  Measured, bf16: 20736 tokens
-// of 32 heads of 128 55 us (6.1 TB/s), 15285 tokens of 32 + 2 x 8 heads into a cache 70 us (5.4 TB/s).
+// of 32 heads of 128 54 us replayed (6.3 TB/s), 59 call after call or with L2 flushed; 15285 tokens of 32 + 2 x 8 heads into a cache 68 - 71 us (5.5 TB/s).
+// (The 16-bit form with split pairs and without a cache holds 24 bytes of a thread in memory at its 64 registers.)
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -17,7 +18,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxTokens = 16;       // tokens of a block, at most; a power of two
 // Rows of a thread whose loads are in flight together: 4 vectors of 16 bytes twice over are 32 registers; the writing of a cache holds more
-// beside them (16384 tokens of 32 + 2 x 8 heads of 128, bf16: 73 us with 3, 79 with 4; rotary of 20736 x 32 x 128 66 us with 3, 55 with 4).
+// beside them.  With 3 and with 4, us: 15285 tokens of 32 + 2 x 8 heads of 128, bf16 67.8 and 70.9, 4096 of 64-wide heads 10.8 and 12.7, 2048 of 12 + 2 x 12
+// heads of 64, f16 6.5 and 7.4, 64 tokens 4.05 and 4.4; 8192 of 16 + 2 x 4 in f32 37.6 and 35.7.  Rotary of 20736 x 32 x 128 66 and 55.
 template <bool CACHE> constexpr int unrolled() { return CACHE ? 3 : 4; }
 
 struct RotArgs {
@@ -249,7 +251,8 @@ template <typename T, int VEC, bool CACHE>
 int launch(RotArgs& a, cudaStream_t st) {
   constexpr int kUnroll = unrolled<CACHE>();
   // Tokens of a block: a power of two, as many as give every thread kUnroll rows (twice that when it writes a cache, whose lookups are
-  // then shared by more rows: 70 us against 73.5 for 15285 tokens), fewer while the grid has less than two blocks an SM,
+  // then shared by more rows: 15285 tokens of 32 + 2 x 8 heads of 128 67.8 us against 69.3, 8192 of 64 + 2 x 8 61.2 against 68.5, 4096 of 32 + 2 x 8 of 64
+  // 10.8 against 11.3), fewer while the grid has less than two blocks an SM,
   // and no more than shared memory has room for (48 KB without an opt-in).
   a.rows = CACHE ? a.nQ + 2 * a.nK : a.nQ;
   a.perRow = (a.d + 2 * VEC - 1) / (2 * VEC);
