@@ -104,3 +104,29 @@ def test_the_device_status_is_healthy_after_the_calls():
         d["new_v"] = d["new"].clone()
         call(d)
         assert device_status() == 0 and device_status(torch.cuda.current_device()) == 0
+
+
+def test_a_module_that_calls_them_is_compiled_in_pieces():
+    """The package's backend compiles what lies between the calls, which run as they are."""
+    from llcompiler_b200.compiler import LLCompiler
+    from llcompiler_b200.executor import kv_append, paged_attention
+    d = _inputs()
+    torch.manual_seed(0)
+
+    class Layer(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.qkv, self.out = torch.nn.Linear(256, 512), torch.nn.Linear(256, 256)
+
+        def forward(self, x):
+            y = self.qkv(x).view(-1, 8, 64).to(torch.bfloat16)
+            q = kv_append(y[:, 4:6], y[:, 6:], d["k"], d["v"], *d["batch"], q=y[:, :4], inv_freq=d["freq"])
+            return self.out(paged_attention(q, d["k"], d["v"], *d["batch"]).reshape(-1, 256).float())
+
+    layer, x = Layer().to(DEV), torch.randn(3, 256, device=DEV)
+    torch._dynamo.reset()
+    with torch.no_grad():
+        want = layer(x)
+        got = torch.compile(layer, backend=LLCompiler())(x)
+    # the projections may differ in their last bits, so that q, k, v and the context round to the neighbouring bf16 number: a step of 2^-8 each
+    assert float((got - want).norm() / want.norm()) < 4 * 2.0 ** -8
