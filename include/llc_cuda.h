@@ -219,7 +219,8 @@ int llc_cuda_kv_append(const LlcKvAppendParams* p, void* stream);
  * batch over a paged cache that holds their keys and values already (llc_cuda_kv_append); query head h reads key head
  * h / (heads / kv_heads).  A token at place p sees the keys j <= p; with window > 0 only those with p - j < window, and the
  * first `sinks` keys of the sequence besides.  A token that sees nothing (kv_len smaller than its place asks for) gets zeros; one
- * whose visible scores are all -inf gets NaN, which is what softmax makes of them.
+ * whose visible scores are all -inf gets NaN, which is what softmax makes of them.  A visible value that is infinite makes its element of the
+ * result infinite, or NaN where its weight is too small for the type it is held in (below about 2^-31 of the largest in f16, 2^-126 otherwise).
  * A slot whose page number is outside [0, num_pages) reads as zeros (key and value) and each such page that a query sees is
  * counted in *bad_pages (at least once, or more often) when that is not NULL.  Nothing else of the cache is read into the
  * result: slots past kv_len, pages before the window and unused pages may hold anything.

@@ -294,3 +294,30 @@ def test_rows_that_see_plus_infinity_are_nan(form):
             k[int(table[0, 0]), 0] = float("-inf")
         got = _run(q, k, v, table, q_start, kv_len, max_q=max(new))
         _against_definition(got, q, k, v, table, q_start, kv_len)
+
+
+def test_chunks_single_tokens_and_matrix_products_at_once():
+    """Calls on streams of their own share SMs, tensor memory and the allocator: each gives what it gives alone."""
+    import gpu_ops as G
+    calls = []
+    for new, lens, heads, kv_heads, d, page, dtype in (FORMS["chunk_whole_blocks"], FORMS["chunk_cut"], FORMS["chunk_cut_d64"], FORMS["decode_cut"], FORMS["decode"]):
+        from llcompiler_b200.executor import paged_attention
+        dev = [R.to_device(t, DEV) for t in (_q(sum(new), heads, d, dtype), *R.make_batch(new, lens, page, kv_heads, d, dtype))]
+        calls.append(lambda dev=dev, n=max(new): paged_attention(*dev, max_q=n))
+    a, b = (torch.randn(512, 512, generator=torch.Generator().manual_seed(i)).to(DEV, torch.bfloat16) for i in range(2))
+
+    def product():
+        y = torch.empty(512, 512, device=DEV, dtype=torch.bfloat16)
+        G.gemm(a[None, None], b.t()[None, None], y[None, None], prec="bf16")
+        return y
+    calls.append(product)
+    alone = [c() for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[] for _ in calls]
+    for _ in range(20):
+        for i, (c, st) in enumerate(zip(calls, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(c())
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for gs, want in zip(got, alone) for g in gs)
